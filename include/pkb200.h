@@ -258,6 +258,70 @@ int pkb200_attention_prefill_kv_append(const void* Q, const void* K_new, const v
                                        int S_q, int S_cache, int S_max, int D, float scale,
                                        int causal, void* stream);
 
+/* ---- paged serving: rotary positions, a paged key/value cache, attention over
+ * it. New entry points; the reference has one contiguous cache of one length
+ * (kv_cache_update.cu:67-69) and no rotary positions.
+ *
+ * Value types of these entry points. */
+enum { PKB200_BF16 = 0, PKB200_FP16 = 1, PKB200_FP32 = 2 };
+
+/* A key/value cache shared out in pages of page_size token rows: pools
+ * [num_pages, heads, page_size, dim] of any strides whose last axis is
+ * contiguous. Strides are in values: {page, head, row}. */
+typedef struct {
+  void* k;
+  void* v;
+  long long k_stride[3];
+  long long v_stride[3];
+  int num_pages, heads, page_size, dim;
+  int dtype; /* PKB200_BF16 or PKB200_FP16 */
+} pkb200_paged_cache;
+
+/* A ragged batch of new tokens (all arrays in device memory). The new tokens of
+ * sequence b are rows [cu_seqlens[b], cu_seqlens[b+1]) of the packed tensors and
+ * the last of its seq_lens[b] tokens; its token p lives in row p % page_size of
+ * page page_table[b * table_stride + p / page_size]. Rows from
+ * cu_seqlens[num_seqs] on belong to no sequence and are left as they were.
+ * The lengths are read on the device only, so a captured graph follows them.
+ * What does not fit (a page outside the pool or the table, offsets out of
+ * order, fewer tokens in a sequence than new ones) is never read or written out of
+ * range: such tokens are not appended, keys of such pages read as zeros, tokens
+ * before position 0 see no key, and the device error word
+ * (pkb200_device_error) becomes 8. */
+typedef struct {
+  const int* page_table; /* [num_seqs, table_width] */
+  const int* cu_seqlens; /* [num_seqs + 1] */
+  const int* seq_lens;   /* [num_seqs], new tokens included */
+  long long table_stride;
+  int table_width, num_seqs;
+  int num_tokens; /* rows of the packed tensors */
+} pkb200_paged_batch;
+
+/* Rotary positions: y = x with the first 2 * rot_pairs values of each head row
+ * rotated in pairs (i, rot_pairs + i), or (2i, 2i + 1) if interleaved, by the
+ * angle positions[b * positions_stride + t] * inv_freq[i] (formed in 64 bits)
+ * and scaled by factor; the other values are copied. backward != 0 rotates by
+ * the negative angle: the gradient with respect to x. x and y are
+ * [B, tokens, H, D] of the given strides ({batch, token, head}, in values, last
+ * axis contiguous); y may be x. |positions| up to 2^31. */
+int pkb200_rope(const void* x, void* y, int dtype, const long long* positions,
+                long long positions_stride, const float* inv_freq, int rot_pairs, int B,
+                long long tokens, int H, int D, const long long* x_strides,
+                const long long* y_strides, float factor, int interleaved, int backward,
+                void* stream);
+
+/* Writes the batch's new rows k, v [num_tokens, heads, dim] (strides {token,
+ * head}, the cache's type) into the cache. With rot_pairs > 0 k is rotated by
+ * the position that each token takes (as pkb200_rope), and so is q
+ * [num_tokens, q_heads, dim] into q_out (which may be q); q_heads may be 0.
+ * Two new tokens that the page table puts in one row leave either's values. */
+int pkb200_paged_kv_append(const pkb200_paged_cache* cache, const pkb200_paged_batch* batch,
+                           const void* k, const long long* k_strides, const void* v,
+                           const long long* v_strides, const void* q, const long long* q_strides,
+                           void* q_out, const long long* q_out_strides, int q_heads,
+                           const float* inv_freq, int rot_pairs, float factor, int interleaved,
+                           void* stream);
+
 /* Caps the grid of the persistent tensor-core GEMM at max_ctas CTAs (one per
  * SM); 0 restores the default of one CTA per SM. Process-wide. The GEMM holds
  * every SM it is given until it finishes, so a tensor-parallel caller that

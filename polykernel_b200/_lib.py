@@ -63,6 +63,10 @@ SIGNATURES = {
     "pkb200_kv_cache_update": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
     "pkb200_attention_prefill_kv_append": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int,
                                                    c_int, c_int, c_int, c_float, c_int, _P]),
+    "pkb200_rope": (c_int, [_P, _P, c_int, _P, c_longlong, _P, c_int, c_int, c_longlong, c_int,
+                            c_int, _P, _P, c_float, c_int, c_int, _P]),
+    "pkb200_paged_kv_append": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, _P, c_int,
+                                       c_float, c_int, _P]),
     "pkb200_set_gemm_max_ctas": (c_int, [c_int]),
     "pkb200_device_arch": (c_int, [ctypes.c_char_p, c_size_t]),
     "pkb200_tuning_load": (c_int, [ctypes.c_char_p, ctypes.c_char_p, c_size_t]),
@@ -80,6 +84,22 @@ SIGNATURES = {
     "pkb200_mlp_block_rmsnorm_next": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int,
                                               c_int, c_float, c_float, _P, c_size_t, _P]),
 }
+
+
+
+class PagedCache(ctypes.Structure):
+    """pkb200_paged_cache."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_stride", c_longlong * 3),
+                ("v_stride", c_longlong * 3), ("num_pages", c_int), ("heads", c_int),
+                ("page_size", c_int), ("dim", c_int), ("dtype", c_int)]
+
+
+class PagedBatch(ctypes.Structure):
+    """pkb200_paged_batch."""
+    _fields_ = [("page_table", c_void_p), ("cu_seqlens", c_void_p), ("seq_lens", c_void_p),
+                ("table_stride", c_longlong), ("table_width", c_int), ("num_seqs", c_int),
+                ("num_tokens", c_int)]
+
 
 _lib = None
 

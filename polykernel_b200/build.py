@@ -7,16 +7,23 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "_lib", "libpkb200.so")
+SOURCES = ["pkb200", "paged"]
 
 
 def build(verbose: bool = False) -> str:
     os.makedirs(os.path.dirname(OUT), exist_ok=True)
-    cmd = ["nvcc", "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17",
-           "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-shared",
-           "-o", OUT, os.path.join(CSRC, "pkb200.cu"), "-lcudart"]
+    arch = ["nvcc", "-gencode", "arch=compute_100a,code=sm_100a"]
+    flags = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC"]
+    objects = [os.path.join(os.path.dirname(OUT), name + ".o") for name in SOURCES]
+    steps = [arch + flags + ["-c", "-o", obj, os.path.join(CSRC, name + ".cu")]
+             for name, obj in zip(SOURCES, objects)]
+    link = arch + ["-Xcompiler", "-fPIC", "-shared", "-o", OUT, *objects, "-lcudart"]
     if verbose:
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True, cwd=CSRC)
+        print("\n".join(" ".join(cmd) for cmd in steps + [link]))
+    running = [subprocess.Popen(cmd, cwd=CSRC) for cmd in steps]  # side by side
+    if any([p.wait() for p in running]):
+        raise RuntimeError("pkb200: nvcc failed")
+    subprocess.run(link, check=True, cwd=CSRC)
     # the .npy launcher harness (reference cuda_run command line) over the library
     harness = ["nvcc", "-Wno-deprecated-gpu-targets", "-O2", "-std=c++17", "-o", os.path.join(os.path.dirname(OUT), "cuda_run"),
                os.path.join(CSRC, "cuda_run.cpp"), "-L" + os.path.dirname(OUT), "-lpkb200",

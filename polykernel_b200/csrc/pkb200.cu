@@ -22,6 +22,7 @@
 #include "attention_tc.cuh"
 #include "gemm_tc2.cuh"
 #include "fp8.cuh"
+#include "internal.h"
 #include "simt_kernels.cuh"
 #include "tuning.h"
 #include "../../include/pkb200.h"
@@ -1026,6 +1027,27 @@ int tp_ce_step(TpCePlan* pl, const bf16* h, const bf16* xn, const bf16* w1, cons
 }
 
 }  // namespace
+
+namespace pkb200 {
+namespace internal {
+
+int device(int* sms, int** err) {
+  DeviceInfo* di = nullptr;
+  const int e = current_device_info(&di);
+  if (e) return e;
+  *sms = di->sms;
+  *err = di->err;
+  return cudaSuccess;
+}
+int smem_attr(const void* func, int smem) { return ensure_smem_attr(func, smem); }
+bool tensor_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,
+                const cuuint64_t* dims, const cuuint64_t* strides_bytes, const cuuint32_t* box) {
+  return make_map(map, type, rank, base, dims, strides_bytes, box);
+}
+void count_launch(LaunchKind kind) { g_counters[kind]++; }
+
+}  // namespace internal
+}  // namespace pkb200
 
 // =================================================================== C ABI ==
 extern "C" {

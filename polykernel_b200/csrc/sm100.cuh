@@ -30,6 +30,7 @@ enum DeviceError : int {
   kErrAbortSeen = 5,        // a role saw another role's abort
   kErrTimeoutSelfTest = 6,  // the wait-timeout self test (a wait nobody satisfies)
   kErrTimeoutConvert = 7,   // attention V-tile converter waited too long
+  kErrBadBatch = 8,         // a paged batch names a page, row or length out of range
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -174,6 +175,15 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
 
@@ -448,6 +458,17 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+
+// ------------------------------------------------- programmatic launches --
+// A kernel launched with programmatic stream serialisation starts while its
+// predecessor still runs; it waits here until the predecessor's writes are
+// visible. The predecessor lets it start early with launch_dependents.
+__device__ __forceinline__ void grid_dependency_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void grid_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 // ------------------------------------------------------------ bf16 helpers --

@@ -395,3 +395,8 @@ def qkv_projection(x, w_qkv, num_heads):
     check(lib().pkb200_qkv_projection(_ptr(x), _ptr(w_qkv), _ptr(q), _ptr(k), _ptr(v), B, S,
                                       num_heads, Dh, _stream()), "qkv_projection")
     return q, k, v
+
+
+# Ragged batches over a paged cache (polykernel_b200/paged.py).
+from .paged import (paged_kv_append, rope, rope_backward,  # noqa: E402,F401
+                    rope_frequencies)
