@@ -322,6 +322,30 @@ int pkb200_paged_kv_append(const pkb200_paged_cache* cache, const pkb200_paged_b
                            const float* inv_freq, int rot_pairs, float factor, int interleaved,
                            void* stream);
 
+/* Attention of a batch's new tokens over their sequences' pages (after
+ * pkb200_paged_kv_append): out = softmax(scale * q k^T) v for q and out
+ * [num_tokens, q_heads, dim] (strides {token, head}), query head h reading key head
+ * h / (q_heads / heads). Token i of a sequence's n new ones is at position
+ * seq_len - n + i; causal: it sees the keys up to its own position, window > 0:
+ * the last `window` of those. lse (may be NULL): fp32 [num_tokens, q_heads], the natural
+ * log of each row's sum of exponentials. A row that sees no key gives zeros
+ * and -inf; keys that a row does not see contribute nothing, whatever values they
+ * hold. dim a multiple of 8 up to 256, page_size a multiple of 8, base addresses
+ * 16-byte aligned and strides multiples of 8 values; scale > 0.
+ * max_q_len: the most new tokens of a sequence. It selects kernels (few rows
+ * per key head, or many) and never changes what is computed.
+ * workspace: caller-owned device memory, 256-byte aligned, of
+ * pkb200_paged_attention_workspace_size bytes for the same arguments; calls that may
+ * overlap on the GPU need their own. */
+size_t pkb200_paged_attention_workspace_size(const pkb200_paged_cache* cache,
+                                             const pkb200_paged_batch* batch, int q_heads,
+                                             int max_q_len, int window);
+int pkb200_paged_attention(const pkb200_paged_cache* cache, const pkb200_paged_batch* batch,
+                           const void* q, const long long* q_strides, void* out,
+                           const long long* out_strides, float* lse, int q_heads, int max_q_len,
+                           int causal, int window, float scale, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 /* Caps the grid of the persistent tensor-core GEMM at max_ctas CTAs (one per
  * SM); 0 restores the default of one CTA per SM. Process-wide. The GEMM holds
  * every SM it is given until it finishes, so a tensor-parallel caller that

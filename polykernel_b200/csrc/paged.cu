@@ -4,6 +4,8 @@
 #include <cmath>
 
 #include "internal.h"
+#include "paged_rows.cuh"
+#include "paged_tiles.cuh"
 #include "rotary.cuh"
 #include "../../include/pkb200.h"
 
@@ -75,6 +77,215 @@ bool batch_ok(const pkb200_paged_batch* b) {
   return b && b->num_seqs >= 0 && b->num_tokens >= 0 && b->table_width >= 0 &&
          (b->num_seqs == 0 ||
           (b->cu_seqlens && b->seq_lens && (b->page_table || b->table_width == 0)));
+}
+
+// ---------------------------------------------------------- attention plan --
+// Which kernels a call of paged attention runs, decided from sizes that the host
+// knows: lengths live on the device, so every kernel takes any lengths, and
+// max_q_len only says which kernel is the faster one for them.
+struct Plan {
+  int dp = 0;         // head width of the kernels: 64, 128 or 256
+  int rows_mr = 0;    // row tile of the rows kernel, 0: not launched
+  int rows_max = 0;   // sequences that it takes: those of at most so many rows
+  int rows_grid = 0;
+  bool tiles = false;  // tile kernel, for the sequences above rows_max
+  int tiles_n = 0, splits = 1;
+  size_t rows_o = 0, rows_ml = 0, rows_meta = 0, tiles_o = 0, tiles_ml = 0, tiles_meta = 0, bytes = 0;
+};
+
+// Rows (new tokens x heads of a group) up to which the rows kernel takes a
+// sequence when all are that short: its four 16-row warps.
+constexpr int kRowsMost = 64;
+constexpr int kRowsMinUnits = 2, kTilesMinUnits = 4;
+
+size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+
+Plan make_plan(const pkb200_paged_cache* c, const pkb200_paged_batch* b, int q_heads, int max_q_len,
+               int window, int sms) {
+  Plan pl;
+  const int G = q_heads / c->heads;
+  pl.dp = c->dim <= 64 ? 64 : c->dim <= 128 ? 128 : 256;
+  const long long T = b->num_tokens, B = b->num_seqs;
+  const long long most = max_q_len < T ? max_q_len : T;
+  const long long rows = most * G;  // of the longest sequence
+  const bool tiles_can = pl.dp <= 128 && G <= 128;
+  if (rows <= kRowsMost || !tiles_can) {
+    pl.rows_mr = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    pl.rows_max = 0x7fffffff;
+  } else {
+    pl.tiles = true;
+    // Single tokens among the prompts go to the rows kernel, unless the sizes
+    // say that there are none.
+    if (B > 1 && T < B * most && G <= kRowsMost) {
+      pl.rows_mr = G <= 16 ? 16 : G <= 32 ? 32 : 64;
+      pl.rows_max = pl.rows_mr;
+    }
+  }
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t o = at;
+    at += up256(n);
+    return o;
+  };
+  if (pl.rows_mr) {
+    pl.rows_grid = sms * (pl.dp <= 128 ? 2 : 1);
+    const size_t slots = 2 * static_cast<size_t>(pl.rows_grid) + 2;
+    pl.rows_o = take(slots * pl.rows_mr * pl.dp * 4);
+    pl.rows_ml = take(slots * pl.rows_mr * 8);
+    pl.rows_meta = take(static_cast<size_t>(pl.rows_grid) * sizeof(paged::Entry));
+  }
+  if (pl.tiles) {
+    const long long per = 2 * (128 / G);  // tokens of a block
+    const long long n = (T + B * (per - 1)) / per;
+    const long long blocks = n * c->heads;
+    // Split the keys where that fills the SMs better: time in key tiles of the
+    // last block to finish, with 8 tiles' worth for a block's start and end.
+    long long units = (static_cast<long long>(b->table_width) * c->page_size + 127) / 128;
+    if (window > 0 && units > (window + per) / 128 + 2) units = (window + per) / 128 + 2;
+    double best = 0;
+    for (int s = 1; s <= 64; ++s) {
+      if (s > 1 && (s * kTilesMinUnits > units || blocks * s > 8LL * sms)) break;
+      const double cost = static_cast<double>((blocks * s + sms - 1) / sms) * (static_cast<double>(units) / s + 8);
+      if (s == 1 || cost < 0.93 * best) {
+        best = cost;
+        pl.splits = s;
+      }
+    }
+    pl.tiles_n = static_cast<int>(n);
+    if (pl.splits > 1) {
+      const size_t entries = static_cast<size_t>(blocks), slots = entries * pl.splits;
+      pl.tiles_o = take(slots * 256 * pl.dp * 4);
+      pl.tiles_ml = take(slots * 256 * 8);
+      pl.tiles_meta = take(entries * sizeof(paged::Entry));
+    }
+  }
+  pl.bytes = at;
+  return pl;
+}
+
+bool attention_ok(const pkb200_paged_cache* c, const pkb200_paged_batch* b, int q_heads, int max_q_len) {
+  return cache_ok(c) && batch_ok(b) && q_heads > 0 && q_heads % c->heads == 0 && max_q_len >= 0 &&
+         c->dim % 8 == 0 && c->dim <= 256 && c->page_size % 8 == 0 &&
+         static_cast<long long>(b->num_tokens) * (q_heads / c->heads) < 0x7fffffffLL;
+}
+
+// Map of a pool [pages, heads, rows, dim] with boxes of 64 values x `box` rows.
+bool pool_map(CUtensorMap* m, const pkb200_paged_cache* c, const void* base, const long long* st, int box) {
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c->dim), static_cast<cuuint64_t>(c->page_size),
+                              static_cast<cuuint64_t>(c->heads), static_cast<cuuint64_t>(c->num_pages)};
+  // the stride of an axis of one is never taken, but has to be a legal one
+  const cuuint64_t row = static_cast<cuuint64_t>(c->dim) * 2;
+  const cuuint64_t strides[3] = {c->page_size > 1 ? static_cast<cuuint64_t>(st[2]) * 2 : row,
+                                 c->heads > 1 ? static_cast<cuuint64_t>(st[1]) * 2 : row,
+                                 c->num_pages > 1 ? static_cast<cuuint64_t>(st[0]) * 2 : row};
+  const cuuint32_t bx[4] = {64, static_cast<cuuint32_t>(box), 1, 1};
+  return internal::tensor_map(m, c->dtype == PKB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                              4, base, dims, strides, bx);
+}
+
+// The largest power of two that divides the page size, up to `most`.
+int box_for(int page_size, int most) {
+  int box = most;
+  while (page_size % box) box >>= 1;
+  return box;
+}
+
+// Launches the joining pass so that it may start while the attention kernel drains.
+template <typename T, int DP>
+int launch_join(const paged::AttnParams& a, int entries, int slot_rows, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(entries, (slot_rows + 3) / 4);
+  cfg.blockDim = dim3(paged::kJoinThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged::paged_join_kernel<T, DP>, a, slot_rows);
+  internal::count_launch(internal::kOther);
+  return e;
+}
+
+template <typename T, int DP, int MR>
+int launch_rows(const pkb200_paged_cache* c, paged::AttnParams a, const Plan& pl, char* ws, cudaStream_t s) {
+  using C = paged::RowsCfg<DP, MR>;
+  const auto kernel = paged::paged_rows_kernel<T, DP, MR>;
+  if (const int e = internal::smem_attr(reinterpret_cast<const void*>(kernel), C::SMEM)) return e;
+  CUtensorMap mk, mv;
+  a.box = box_for(c->page_size, C::KT);
+  if (!pool_map(&mk, c, c->k, c->k_stride, a.box) || !pool_map(&mv, c, c->v, c->v_stride, a.box))
+    return cudaErrorInvalidValue;
+  a.min_rows = 1;
+  a.max_rows = pl.rows_max;
+  a.min_units = kRowsMinUnits;
+  a.part_o = reinterpret_cast<float*>(ws + pl.rows_o);
+  a.part_ml = reinterpret_cast<float2*>(ws + pl.rows_ml);
+  a.meta = reinterpret_cast<int*>(ws + pl.rows_meta);
+  kernel<<<pl.rows_grid, C::kThreads, C::SMEM, s>>>(mk, mv, a);
+  internal::count_launch(internal::kOther);
+  if (const int e = cudaGetLastError()) return e;
+  return launch_join<T, DP>(a, pl.rows_grid, MR, s);
+}
+
+template <typename T, int DP>
+int launch_tiles(const pkb200_paged_cache* c, paged::AttnParams a, const Plan& pl, char* ws, cudaStream_t s) {
+  using C = paged::TilesCfg<DP>;
+  const auto kernel = paged::paged_tiles_kernel<T, DP>;
+  if (const int e = internal::smem_attr(reinterpret_cast<const void*>(kernel), C::SMEM)) return e;
+  CUtensorMap mq, mk, mv;
+  a.box = box_for(c->page_size, C::KT);
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.D), static_cast<cuuint64_t>(a.Hq),
+                              static_cast<cuuint64_t>(a.T)};
+  const cuuint64_t row = static_cast<cuuint64_t>(a.D) * 2;
+  const cuuint64_t strides[2] = {a.Hq > 1 ? static_cast<cuuint64_t>(a.qs_h) * 2 : row,
+                                 a.T > 1 ? static_cast<cuuint64_t>(a.qs_t) * 2 : row};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.G), static_cast<cuuint32_t>(128 / a.G)};
+  if (!internal::tensor_map(&mq, c->dtype == PKB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                         : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                            3, a.q, dims, strides, box) ||
+      !pool_map(&mk, c, c->k, c->k_stride, a.box) || !pool_map(&mv, c, c->v, c->v_stride, a.box))
+    return cudaErrorInvalidValue;
+  a.min_rows = pl.rows_mr ? pl.rows_max + 1 : 1;
+  a.max_rows = 0x7fffffff;
+  a.min_units = kTilesMinUnits;
+  a.tiles = pl.tiles_n;
+  a.splits = pl.splits;
+  if (pl.splits > 1) {
+    a.part_o = reinterpret_cast<float*>(ws + pl.tiles_o);
+    a.part_ml = reinterpret_cast<float2*>(ws + pl.tiles_ml);
+    a.meta = reinterpret_cast<int*>(ws + pl.tiles_meta);
+  }
+  const long long entries = static_cast<long long>(pl.tiles_n) * a.Hkv;
+  if (entries * pl.splits > 0x7fffffffLL) return cudaErrorInvalidValue;
+  kernel<<<static_cast<unsigned>(entries * pl.splits), C::kThreads, C::SMEM, s>>>(mq, mk, mv, a);
+  internal::count_launch(internal::kAttnTensor);
+  if (const int e = cudaGetLastError()) return e;
+  return pl.splits > 1 ? launch_join<T, DP>(a, static_cast<int>(entries), 256, s) : 0;
+}
+
+template <typename T, int DP>
+int launch_attention(const pkb200_paged_cache* c, const paged::AttnParams& a, const Plan& pl, char* ws,
+                     cudaStream_t s) {
+  if (pl.rows_mr) {
+    const int e = pl.rows_mr == 16   ? launch_rows<T, DP, 16>(c, a, pl, ws, s)
+                  : pl.rows_mr == 32 ? launch_rows<T, DP, 32>(c, a, pl, ws, s)
+                                     : launch_rows<T, DP, 64>(c, a, pl, ws, s);
+    if (e) return e;
+  }
+  if constexpr (DP <= 128) {
+    if (pl.tiles) return launch_tiles<T, DP>(c, a, pl, ws, s);
+  }
+  return 0;
+}
+
+template <typename T>
+int launch_attention(const pkb200_paged_cache* c, const paged::AttnParams& a, const Plan& pl, char* ws,
+                     cudaStream_t s) {
+  return pl.dp == 64    ? launch_attention<T, 64>(c, a, pl, ws, s)
+         : pl.dp == 128 ? launch_attention<T, 128>(c, a, pl, ws, s)
+                        : launch_attention<T, 256>(c, a, pl, ws, s);
 }
 
 }  // namespace
@@ -201,6 +412,76 @@ int pkb200_paged_kv_append(const pkb200_paged_cache* cache, const pkb200_paged_b
   else launch_append<__half>(p, grid, S(stream), a);
   internal::count_launch(internal::kOther);
   return cudaGetLastError();
+}
+
+size_t pkb200_paged_attention_workspace_size(const pkb200_paged_cache* cache,
+                                             const pkb200_paged_batch* batch, int q_heads,
+                                             int max_q_len, int window) {
+  if (!attention_ok(cache, batch, q_heads, max_q_len) || batch->num_tokens == 0 || batch->num_seqs == 0)
+    return 0;
+  int sms, *err;
+  if (internal::device(&sms, &err)) return 0;
+  return make_plan(cache, batch, q_heads, max_q_len, window, sms).bytes;
+}
+
+int pkb200_paged_attention(const pkb200_paged_cache* cache, const pkb200_paged_batch* batch,
+                           const void* q, const long long* q_strides, void* out,
+                           const long long* out_strides, float* lse, int q_heads, int max_q_len,
+                           int causal, int window, float scale, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  if (!attention_ok(cache, batch, q_heads, max_q_len) || window < 0 || (window && !causal) ||
+      !(scale > 0.f) || !std::isfinite(scale))
+    return cudaErrorInvalidValue;
+  if (batch->num_tokens == 0 || batch->num_seqs == 0) return cudaSuccess;
+  if (!q || !out || !q_strides || !out_strides || cache->num_pages == 0) return cudaErrorInvalidValue;
+  for (const void* x : {static_cast<const void*>(cache->k), static_cast<const void*>(cache->v), q,
+                        static_cast<const void*>(out)})
+    if (reinterpret_cast<uintptr_t>(x) & 15u) return cudaErrorInvalidValue;
+  for (int i = 0; i < 3; ++i)
+    if (cache->k_stride[i] % 8 || cache->v_stride[i] % 8) return cudaErrorInvalidValue;
+  for (int i = 0; i < 2; ++i)
+    if (q_strides[i] % 8 || out_strides[i] % 8) return cudaErrorInvalidValue;
+  int sms, *err;
+  if (const int e = internal::device(&sms, &err)) return e;
+  const Plan pl = make_plan(cache, batch, q_heads, max_q_len, window, sms);
+  if (workspace_bytes < pl.bytes || (pl.bytes && !workspace)) return cudaErrorInvalidValue;
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return cudaErrorInvalidValue;
+  paged::AttnParams a = {};
+  a.q = q;
+  a.out = out;
+  a.lse = lse;
+  a.k = cache->k;
+  a.v = cache->v;
+  a.qs_t = q_strides[0];
+  a.qs_h = q_strides[1];
+  a.os_t = out_strides[0];
+  a.os_h = out_strides[1];
+  a.kp_p = cache->k_stride[0];
+  a.kp_h = cache->k_stride[1];
+  a.kp_r = cache->k_stride[2];
+  a.vp_p = cache->v_stride[0];
+  a.vp_h = cache->v_stride[1];
+  a.vp_r = cache->v_stride[2];
+  a.table = batch->page_table;
+  a.table_stride = batch->table_stride;
+  a.cu = batch->cu_seqlens;
+  a.lens = batch->seq_lens;
+  a.B = batch->num_seqs;
+  a.T = batch->num_tokens;
+  a.Hq = q_heads;
+  a.Hkv = cache->heads;
+  a.G = q_heads / cache->heads;
+  a.D = cache->dim;
+  a.page_size = cache->page_size;
+  a.num_pages = cache->num_pages;
+  a.table_width = batch->table_width;
+  a.causal = causal;
+  a.window = window;
+  a.scale_log2 = scale * 1.4426950408889634f;  // log2(e)
+  a.err = err;
+  char* ws = static_cast<char*>(workspace);
+  return cache->dtype == PKB200_BF16 ? launch_attention<__nv_bfloat16>(cache, a, pl, ws, S(stream))
+                                     : launch_attention<__half>(cache, a, pl, ws, S(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,220 @@
+// paged_common.cuh - what the kernels of attention over a paged cache share:
+// the batch description, its sequences' key ranges, and the final pass that
+// joins the pieces of rows whose keys several blocks went over.
+//
+// For a new token at position p of a sequence of `len` tokens and a query head h
+// of key head h / G:
+//   o = sum_j softmax_j(scale * q . k_j) v_j  over the keys j that it sees:
+//   j < len, j <= p if causal, j > p - window if a window is set.
+// Rows of a sequence are numbered token * G + (head in the group), so one tile
+// of rows shares its keys: the G heads of a few tokens.
+//
+// Statistics (running maximum, in log2 units, and sum) and the accumulated
+// output are fp32 in every kernel. A row that sees no key gives zeros and a
+// log-sum of -inf.
+#pragma once
+
+#include <type_traits>
+
+#include "paged_index.h"
+#include "sm100.cuh"
+
+namespace pkb200 {
+namespace paged {
+
+struct AttnParams {
+  const void* q;
+  void* out;
+  float* lse;  // [T, Hq], or null
+  const void* k;
+  const void* v;
+  long long qs_t, qs_h, os_t, os_h;
+  long long kp_p, kp_h, kp_r, vp_p, vp_h, vp_r;  // page, head and row strides of the pools
+  const int* table;
+  long long table_stride;
+  const int* cu;
+  const int* lens;
+  int B, T, Hq, Hkv, G, D, page_size, num_pages, table_width;
+  int causal, window;  // window 0: none
+  float scale_log2;    // scale * log2(e)
+  int box;             // keys of one TMA box: divides the page size and the key tile
+  int min_rows, max_rows;  // this launch takes the sequences with that many rows
+  int min_units;       // least key tiles of a piece of work
+  int splits, tiles;   // tile kernel: pieces of a row tile's keys, bound on row tiles
+  float* part_o;       // [slot][rows][DP] partial outputs, not divided by their sums
+  float2* part_ml;     // [slot][rows] their maxima and sums
+  int* meta;           // [entry][8], see Entry
+  int* err;
+};
+
+// A tile of rows whose pieces the joining pass adds up.
+struct Entry {
+  int pieces;  // 0: nothing to join
+  int t0, hk, row0, rows;
+  int slot0, slot1, step;  // piece k is in slot0, or slot1 + (k - 1) * step
+};
+static_assert(sizeof(Entry) == 32, "");
+
+// Sequence b of the batch.
+__device__ __forceinline__ Seq load_seq(const AttnParams& p, int b, bool report = false) {
+  bool bad;
+  const Seq s = clip_seq(__ldg(p.cu + b), __ldg(p.cu + b + 1), __ldg(p.lens + b), p.T,
+                         static_cast<long long>(p.table_width) * p.page_size, bad);
+  if (report && bad) atomicCAS(p.err, 0, kErrBadBatch);
+  return s;
+}
+__device__ __forceinline__ int key_hi(const AttnParams& p, const Seq& s, int i) {
+  return clip_hi(s, i, p.causal);
+}
+__device__ __forceinline__ int key_lo(const AttnParams& p, const Seq& s, int i) {
+  return clip_lo(s, i, p.window);
+}
+template <int KT>
+__device__ __forceinline__ int key_tiles(const AttnParams& p, const Seq& s, int first, int last,
+                                         int& tile0) {
+  return clip_tiles(s, first, last, p.causal, p.window, KT, tile0);
+}
+
+// The pool page that holds key `key` (below the sequence's length) of sequence
+// b, or num_pages for a page outside the pool.
+__device__ __forceinline__ int page_of(const AttnParams& p, int b, int key) {
+  const int page = clip_page(__ldg(p.table + b * p.table_stride + key / p.page_size), p.num_pages);
+  if (page == p.num_pages) atomicCAS(p.err, 0, kErrBadBatch);
+  return page;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) { return unpack_bf16x2(v); }
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return unpack_f16x2(v); }
+
+// Whether one of the two values in `w` is infinite or NaN (all exponent bits set).
+template <typename T>
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+  constexpr uint32_t e = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+// Weight of a part whose maximum is m within a row whose maximum is top.
+__device__ __forceinline__ float part_weight(float m, float top) {
+  return m == top ? 1.f : fast_exp2(m - top);
+}
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ float log_sum(float m, float l) {
+  constexpr float kLn2 = 0.69314718055994531f;
+  return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+// Position of a sequence of work items in a batch: inclusive sum of `mine` over
+// the block's threads before this one, and the block's total.
+template <int THREADS>
+__device__ __forceinline__ long long block_prefix(long long mine, long long* warp_sums,
+                                                  long long& total) {
+  const int lane = lane_id(), warp = warp_id();
+  long long x = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  long long before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += warp_sums[w];
+    total += warp_sums[w];
+  }
+  return before + x - mine;
+}
+
+// ------------------------------------------------------------------- join --
+// Adds up the pieces of row tiles whose keys several blocks went over: 4 rows
+// per block, 4 warps to a row, each taking every fourth piece. The order of the
+// sums is fixed, so results do not depend on timing. Launched to overlap the
+// attention kernel's tail (grid_dependency_wait).
+constexpr int kJoinThreads = 512;
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttnParams p, int slot_rows) {
+  constexpr int C = (DP + 127) / 128;  // float4 per lane
+  __shared__ float4 o_s[3][4][32 * C];
+  __shared__ float2 ml_s[3][4];
+  grid_dependency_wait();
+  const Entry e = reinterpret_cast<const Entry*>(p.meta)[blockIdx.x];
+  const int warp = warp_id(), lane = lane_id();
+  const int row = static_cast<int>(blockIdx.y) * 4 + (warp & 3);
+  const int part = warp >> 2;
+  if (e.pieces == 0 || static_cast<int>(blockIdx.y) * 4 >= e.rows) return;
+  float m = -INFINITY, l = 0.f;
+  float4 o[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float mk, float lk, const float4 (&ok)[C]) {
+    const float top = fmaxf(m, mk);
+    const float a = part_weight(m, top), b = part_weight(mk, top);
+    m = top;
+    l = l * a + lk * b;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      o[c].x = o[c].x * a + ok[c].x * b;
+      o[c].y = o[c].y * a + ok[c].y * b;
+      o[c].z = o[c].z * a + ok[c].z * b;
+      o[c].w = o[c].w * a + ok[c].w * b;
+    }
+  };
+  if (row < e.rows) {
+#pragma unroll 4
+    for (int k = part; k < e.pieces; k += 4) {
+      const long long at = static_cast<long long>(k == 0 ? e.slot0 : e.slot1 + (k - 1) * e.step) * slot_rows + row;
+      const float2 ml = p.part_ml[at];
+      float4 ok[C];
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int d = lane * 4 + c * 128;
+        ok[c] = d < DP ? *reinterpret_cast<const float4*>(p.part_o + at * DP + d)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      add(ml.x, ml.y, ok);
+    }
+  }
+  if (part > 0) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) o_s[part - 1][warp & 3][c * 32 + lane] = o[c];
+    if (lane == 0) ml_s[part - 1][warp & 3] = make_float2(m, l);
+  }
+  __syncthreads();
+  if (part > 0 || row >= e.rows) return;
+  for (int w = 0; w < 3; ++w) {
+    float4 ok[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) ok[c] = o_s[w][warp][c * 32 + lane];
+    const float2 ml = ml_s[w][warp];
+    add(ml.x, ml.y, ok);
+  }
+  const int r = e.row0 + row;
+  const long long t = e.t0 + r / p.G;
+  const int h = e.hk * p.G + r % p.G;
+  const float inv = inverse_sum(l);
+  T* dst = static_cast<T*>(p.out) + t * p.os_t + h * p.os_h;
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int d = lane * 4 + c * 128;
+    if (d < p.D)
+      *reinterpret_cast<uint2*>(dst + d) =
+          make_uint2(pack2<T>(o[c].x * inv, o[c].y * inv), pack2<T>(o[c].z * inv, o[c].w * inv));
+  }
+  if (p.lse && lane == 0) p.lse[t * p.Hq + h] = log_sum(m, l);
+}
+
+}  // namespace paged
+}  // namespace pkb200

@@ -1,0 +1,574 @@
+// paged_rows.cuh - attention over a paged cache for few rows per key head:
+// single tokens, drafted tokens, small groups of heads (sm_100a).
+//
+// Bound by reading every visible key and value once from HBM, so the work is
+// split by keys: all 64-key tiles of the batch, over (sequence, key head, row
+// tile), form one line that the grid cuts into equal runs, whatever the lengths
+// are. A block that covers a row tile's keys from end to end writes the
+// output; otherwise pieces go to the workspace (at most two per block: the
+// tail of the tile it starts in and the head of the one it ends in) and
+// paged_join_kernel adds them up. The lengths are read on the device.
+//
+// One warp per block fetches pages by TMA into a ring of key and value tiles;
+// four warps work on them with mma.sync (M = 16 rows: a tcgen05 tile would be
+// 7/8 empty, and the tensor work is a small part of the time of the reads).
+// With MR = 16 rows each warp takes 16 of a tile's 64 keys with statistics of
+// its own, merged at the end of the row tile; with MR = 32 or 64 two or all
+// four warps take different rows. P enters the P.V product as two 16-bit terms
+// (value and remainder), so the output carries no rounding of P: the second
+// product costs nothing that the reads do not hide.
+#pragma once
+
+#include "paged_common.cuh"
+
+namespace pkb200 {
+namespace paged {
+
+template <int DP, int MR>
+struct RowsCfg {
+  static constexpr int KT = 64;
+  static constexpr int kThreads = 160;  // 4 compute warps, 1 that fetches
+  static constexpr int WM = MR / 16, WK = 4 / WM, KW = KT / WK;  // warps by rows and by keys
+  static constexpr int SLOT = KT * DP * 2;
+  // 80 KB in flight per block, two blocks per SM (one with 256-wide heads)
+  static constexpr int kBlocks = DP <= 128 ? 2 : 1;
+  static constexpr int SLOTS = DP == 64 ? 10 : DP == 128 ? 5 : 5;
+  static constexpr int OFF_STAGE = SLOTS * SLOT;  // merge: 2 x 16 rows of fp32
+  static constexpr int STAGE = WK > 1 ? 2 * 16 * DP * 4 : 0;
+  static constexpr int OFF_ML = OFF_STAGE + STAGE;        // float2[4][16]
+  static constexpr int OFF_BAR = OFF_ML + 4 * 16 * 8;     // full[SLOTS], empty[SLOTS]
+  static constexpr int OFF_SCAN = OFF_BAR + 2 * SLOTS * 8;  // long long[5], start of the run
+  static constexpr int SMEM = OFF_SCAN + 5 * 8 + 32 + 1024;
+};
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void compute_warps_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// Place in the line of work: a row tile `rt` of key head `hk` of sequence `b`.
+template <int MR>
+struct RowCursor {
+  const AttnParams& p;
+  int b, hk, rt;
+  Seq s;
+  int rows, row_tiles;  // rows of the sequence
+  int tile0, n;         // key tiles of this row tile
+
+  __device__ explicit RowCursor(const AttnParams& p_) : p(p_) {}
+  __device__ static int rows_of(const AttnParams& p, const Seq& s) {
+    const int rows = s.nq * p.G;
+    return rows >= p.min_rows && rows <= p.max_rows ? rows : 0;
+  }
+  __device__ static int tiles_of(const AttnParams& p, const Seq& s, int rows, int rt, int& tile0) {
+    return key_tiles<64>(p, s, rt * MR / p.G, (min(rows, rt * MR + MR) - 1) / p.G, tile0);
+  }
+  // Key tiles of a whole sequence (one key head).
+  __device__ static long long units_of(const AttnParams& p, const Seq& s) {
+    const int rows = rows_of(p, s);
+    long long n = 0;
+    int tile0;
+    for (int rt = 0; rt * MR < rows; ++rt) n += tiles_of(p, s, rows, rt, tile0);
+    return n;
+  }
+  __device__ void load() {
+    s = load_seq(p, b);
+    rows = rows_of(p, s);
+    row_tiles = (rows + MR - 1) / MR;
+  }
+  // Start in sequence b, `rem` key tiles after its first one; returns the
+  // offset within the row tile.
+  __device__ int start(int b_, long long rem) {
+    b = b_;
+    load();
+    const long long per_head = units_of(p, s);
+    hk = static_cast<int>(rem / per_head);
+    rem -= hk * per_head;
+    for (rt = 0;; ++rt) {
+      n = tiles_of(p, s, rows, rt, tile0);
+      if (rem < n) return static_cast<int>(rem);
+      rem -= n;
+    }
+  }
+  __device__ void next() {
+    if (++rt == row_tiles) {
+      rt = 0;
+      if (++hk == p.Hkv) {
+        hk = 0;
+        do {
+          ++b;
+          load();
+        } while (rows == 0);
+      }
+    }
+    n = tiles_of(p, s, rows, rt, tile0);
+  }
+};
+
+template <typename T, int DP, int MR>
+__global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kBlocks)
+    paged_rows_kernel(const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const AttnParams p) {
+  using C = RowsCfg<DP, MR>;
+  constexpr int KT = C::KT, KW = C::KW, WK = C::WK, SLOTS = C::SLOTS;
+  constexpr int HALVES = DP / 64;  // 128-byte wide columns of a tile
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* empty = full + SLOTS;
+  long long* scan = reinterpret_cast<long long*>(smem + C::OFF_SCAN);
+  long long* start_rem = scan + 5;
+  int* start_b = reinterpret_cast<int*>(scan + 6);
+  volatile int* abort_flag = start_b + 1;
+  const int warp = warp_id(), lane = lane_id();
+  Entry* const meta = reinterpret_cast<Entry*>(p.meta) + blockIdx.x;
+
+  grid_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  // This block's run [u0, u1) of the batch's key tiles.
+  long long u0, u1, per_block;
+  {
+    const int each = (p.B + C::kThreads - 1) / C::kThreads;
+    const int b0 = static_cast<int>(threadIdx.x) * each, b1 = min(p.B, b0 + each);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += p.Hkv * RowCursor<MR>::units_of(p, load_seq(p, b, true));
+    long long total;
+    const long long before = block_prefix<C::kThreads>(mine, scan, total);
+    per_block = max(static_cast<long long>(p.min_units), (total + gridDim.x - 1) / gridDim.x);
+    u0 = blockIdx.x * per_block;
+    u1 = min(total, u0 + per_block);
+    if (u0 >= u1) {
+      if (threadIdx.x == 0) meta->pieces = 0;
+      return;
+    }
+    if (u0 >= before && u0 < before + mine) {
+      long long at = before;
+      for (int b = b0;; ++b) {
+        const long long n = p.Hkv * RowCursor<MR>::units_of(p, load_seq(p, b));
+        if (u0 < at + n) {
+          *start_b = b;
+          *start_rem = u0 - at;
+          break;
+        }
+        at += n;
+      }
+    }
+    __syncthreads();
+  }
+  RowCursor<MR> at(p);
+  int off = at.start(*start_b, *start_rem);
+
+  if (warp == 4) {
+    // ------------------------------------------------------------- fetch --
+    if (lane == 0) {
+      tma_prefetch_desc(&map_k);
+      tma_prefetch_desc(&map_v);
+    }
+    const int boxes = KT / p.box;  // per tile and column
+    const int col = lane / boxes, bx = lane - col * boxes;
+    const bool mine = col < HALVES;
+    int slot = 0, issued = 0;
+    uint32_t parity = 1;
+    bool ok = true;
+    for (long long u = u0; u < u1 && ok;) {
+      const int run = static_cast<int>(min(static_cast<long long>(at.n - off), u1 - u));
+      auto lookup = [&](int tile) {  // this lane's page in that key tile
+        const int key = (at.tile0 + tile) * KT + bx * p.box;
+        return mine && key < at.s.len ? page_of(p, at.b, key) : -1;
+      };
+      int page = lookup(off);
+      for (int i = 0; i < run && ok; ++i) {
+        const int key = (at.tile0 + off + i) * KT + bx * p.box;
+        const int next = i + 1 < run ? lookup(off + i + 1) : -1;
+        const int row = key % p.page_size;
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, page >= 0)) * p.box * 128;
+#pragma unroll
+        for (int kv = 0; kv < 2 && ok; ++kv) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], parity, p.err, abort_flag,
+                                                 kErrTimeoutProducer));
+          if (!ok) break;
+          if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
+          __syncwarp();
+          if (page >= 0)
+            tma_load_4d(smem + slot * C::SLOT + col * (KT * 128) + bx * p.box * 128, kv ? &map_v : &map_k,
+                        &full[slot], col * 64, row, at.hk, page);
+          ++issued;
+          if (++slot == SLOTS) {
+            slot = 0;
+            parity ^= 1;
+          }
+        }
+        page = next;
+      }
+      u += run;
+      off = 0;
+      if (u < u1) at.next();
+    }
+    if (!ok) {  // do not leave while copies into this block's memory are in flight
+      for (int i = max(0, issued - SLOTS); i < issued; ++i) {
+        const long long t0 = clock64();
+        while (!mbar_try_wait(&full[i % SLOTS], (i / SLOTS) & 1) && clock64() - t0 < kSpinLimitCycles) {}
+      }
+    }
+    return;
+  }
+
+  // ----------------------------------------------------------- attention --
+  const int wm = warp / WK, wk = warp % WK;
+  const int g = lane >> 2, t4 = lane & 3;
+  float* stage = reinterpret_cast<float*>(smem + C::OFF_STAGE);
+  float2* ml_s = reinterpret_cast<float2*>(smem + C::OFF_ML);
+  const uint32_t slots_addr = smem_u32(smem);
+  // ldmatrix row addresses of this lane within a tile. K: matrices (keys 0-7,
+  // chunk c), (keys 0-7, c + 1), (keys 8-15, c), (keys 8-15, c + 1); V
+  // (transposed): (keys 0-7, c), (keys 8-15, c), (keys 0-7, c + 1), (keys 8-15, c + 1).
+  const int key_k = wk * KW + (lane & 7) + ((lane >> 4) << 3), chunk_k = (lane >> 3) & 1;
+  const int key_v = wk * KW + (lane & 15), chunk_v = lane >> 4;
+  int slot = 0;
+  uint32_t parity = 0;
+  bool wrote_meta = false;
+  bool ok = true;
+
+  for (long long u = u0; u < u1 && ok;) {
+    const int run = static_cast<int>(min(static_cast<long long>(at.n - off), u1 - u));
+    const int row0 = at.rt * MR + wm * 16;
+    const int ra = min(row0 + g, at.rows - 1), rb = min(row0 + g + 8, at.rows - 1);
+    const int tok_a = ra / p.G, tok_b = rb / p.G;
+    // Q rows (A operand), rows g and g + 8 of this warp
+    uint32_t qf[DP / 16][4];
+    {
+      const T* qa = static_cast<const T*>(p.q) + (at.s.t0 + tok_a) * p.qs_t + (at.hk * p.G + ra - tok_a * p.G) * p.qs_h;
+      const T* qb = static_cast<const T*>(p.q) + (at.s.t0 + tok_b) * p.qs_t + (at.hk * p.G + rb - tok_b * p.G) * p.qs_h;
+#pragma unroll
+      for (int i = 0; i < DP / 16; ++i) {
+        const int d = i * 16 + t4 * 2;
+        qf[i][0] = d < p.D ? *reinterpret_cast<const uint32_t*>(qa + d) : 0u;
+        qf[i][1] = d < p.D ? *reinterpret_cast<const uint32_t*>(qb + d) : 0u;
+        qf[i][2] = d + 8 < p.D ? *reinterpret_cast<const uint32_t*>(qa + d + 8) : 0u;
+        qf[i][3] = d + 8 < p.D ? *reinterpret_cast<const uint32_t*>(qb + d + 8) : 0u;
+      }
+    }
+    const int hi_a = key_hi(p, at.s, tok_a), hi_b = key_hi(p, at.s, tok_b);
+    const int lo_a = key_lo(p, at.s, tok_a), lo_b = key_lo(p, at.s, tok_b);
+    // keys that all rows of the tile see
+    const int all_lo = key_lo(p, at.s, (min(at.rows, at.rt * MR + MR) - 1) / p.G);
+    const int all_hi = key_hi(p, at.s, at.rt * MR / p.G);
+    float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
+    float o[DP / 8][4];
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+
+    for (int i = 0; i < run; ++i) {
+      const int key0 = (at.tile0 + off + i) * KT;
+      // ---- S = Q K^T
+      float s[KW / 8][4];
+#pragma unroll
+      for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], parity, p.err, abort_flag, kErrTimeoutSoftmax));
+      if (!ok) break;
+      {
+        const uint32_t base = slots_addr + slot * C::SLOT;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+#pragma unroll
+          for (int n = 0; n < KW / 16; ++n) {
+            const int key = key_k + n * 16, c = (ks & 3) * 2 + chunk_k;
+            uint32_t kf[4];
+            ldmatrix4(base + (ks >> 2) * (KT * 128) + key * 128 + ((c ^ (key & 7)) << 4), kf);
+            mma16816<T>(s[2 * n], qf[ks], kf[0], kf[1]);
+            mma16816<T>(s[2 * n + 1], qf[ks], kf[2], kf[3]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[slot]);
+      if (++slot == SLOTS) {
+        slot = 0;
+        parity ^= 1;
+      }
+      // ---- softmax
+      const bool masked = key0 + KT > all_hi || key0 < all_lo;
+      if (masked) {
+#pragma unroll
+        for (int n = 0; n < KW / 8; ++n) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int key = key0 + wk * KW + n * 8 + t4 * 2 + c;
+            if (key < lo_a || key >= hi_a) s[n][c] = -INFINITY;
+            if (key < lo_b || key >= hi_b) s[n][2 + c] = -INFINITY;
+          }
+        }
+      }
+      float mx_a = -INFINITY, mx_b = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < KW / 8; ++n) {
+        mx_a = fmaxf(mx_a, fmaxf(s[n][0], s[n][1]));
+        mx_b = fmaxf(mx_b, fmaxf(s[n][2], s[n][3]));
+      }
+#pragma unroll
+      for (int x = 1; x <= 2; x <<= 1) {
+        mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, x));
+        mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, x));
+      }
+      const float new_a = fmaxf(m_a, mx_a * p.scale_log2), new_b = fmaxf(m_b, mx_b * p.scale_log2);
+      if (__any_sync(0xffffffffu, new_a != m_a || new_b != m_b)) {
+        const float fa = part_weight(m_a, new_a), fb = part_weight(m_b, new_b);
+        m_a = new_a;
+        m_b = new_b;
+        l_a *= fa;
+        l_b *= fb;
+#pragma unroll
+        for (int d = 0; d < DP / 8; ++d) {
+          o[d][0] *= fa;
+          o[d][1] *= fa;
+          o[d][2] *= fb;
+          o[d][3] *= fb;
+        }
+      }
+      const float sub_a = m_a == -INFINITY ? 0.f : m_a, sub_b = m_b == -INFINITY ? 0.f : m_b;
+#pragma unroll
+      for (int n = 0; n < KW / 8; ++n) {
+        s[n][0] = fast_exp2(fmaf(s[n][0], p.scale_log2, -sub_a));
+        s[n][1] = fast_exp2(fmaf(s[n][1], p.scale_log2, -sub_a));
+        s[n][2] = fast_exp2(fmaf(s[n][2], p.scale_log2, -sub_b));
+        s[n][3] = fast_exp2(fmaf(s[n][3], p.scale_log2, -sub_b));
+        l_a += s[n][0] + s[n][1];
+        l_b += s[n][2] + s[n][3];
+      }
+      // ---- O += P V
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], parity, p.err, abort_flag, kErrTimeoutSoftmax));
+      if (!ok) break;
+      const uint32_t base = slots_addr + slot * C::SLOT;
+      bool by_hand = false;
+      if (masked) {
+        // A masked key has P = 0, but 0 * inf and 0 * NaN are NaN. Rows past
+        // the sequence's end (stale memory) are cleared here; values of keys
+        // that only some rows see cannot be, and if one of those is not
+        // finite this tile's products are formed one by one.
+        bool bad = false;
+        for (int x = lane; x < KW * HALVES * 8; x += 32) {
+          const int key = wk * KW + x / (HALVES * 8), c = x % (HALVES * 8);
+          uint4* w = reinterpret_cast<uint4*>(smem + slot * C::SLOT + (c >> 3) * (KT * 128) + key * 128 + (c & 7) * 16);
+          if (key0 + key >= at.s.len) *w = make_uint4(0u, 0u, 0u, 0u);
+          else {
+            const uint4 v = *w;
+            bad |= not_finite2<T>(v.x) || not_finite2<T>(v.y) || not_finite2<T>(v.z) || not_finite2<T>(v.w);
+          }
+        }
+        fence_proxy_async_smem();
+        by_hand = __any_sync(0xffffffffu, bad);
+      }
+      if (!by_hand) {
+#pragma unroll
+        for (int kb = 0; kb < KW / 16; ++kb) {
+          uint32_t ph[4], pl[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const float v0 = s[2 * kb + (x >> 1)][(x & 1) * 2], v1 = s[2 * kb + (x >> 1)][(x & 1) * 2 + 1];
+            ph[x] = pack2<T>(v0, v1);
+            const float2 r = unpack2<T>(ph[x]);
+            pl[x] = pack2<T>(v0 - r.x, v1 - r.y);
+          }
+#pragma unroll
+          for (int d = 0; d < DP / 16; ++d) {
+            const int key = key_v + kb * 16, c = (d & 3) * 2 + chunk_v;
+            uint32_t vf[4];
+            ldmatrix4_trans(base + (d >> 2) * (KT * 128) + key * 128 + ((c ^ (key & 7)) << 4), vf);
+            mma16816<T>(o[2 * d], ph, vf[0], vf[1]);
+            mma16816<T>(o[2 * d + 1], ph, vf[2], vf[3]);
+            mma16816<T>(o[2 * d], pl, vf[0], vf[1]);
+            mma16816<T>(o[2 * d + 1], pl, vf[2], vf[3]);
+          }
+        }
+      } else {
+        for (int kk = 0; kk < KW; ++kk) {
+          float pa = 0.f, pb = 0.f;  // this key's P in rows g and g + 8
+#pragma unroll
+          for (int n = 0; n < KW / 8; ++n) {
+            if (n == kk >> 3) {
+              pa = (kk & 1) ? s[n][1] : s[n][0];
+              pb = (kk & 1) ? s[n][3] : s[n][2];
+            }
+          }
+          const int src = (lane & ~3) | ((kk & 7) >> 1);
+          pa = __shfl_sync(0xffffffffu, pa, src);
+          pb = __shfl_sync(0xffffffffu, pb, src);
+          const int k = wk * KW + kk, key = key0 + k;
+          const bool see_a = key >= lo_a && key < hi_a, see_b = key >= lo_b && key < hi_b;
+#pragma unroll
+          for (int d = 0; d < DP / 8; ++d) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(
+                smem + slot * C::SLOT + (d >> 3) * (KT * 128) + k * 128 + (((d & 7) ^ (k & 7)) << 4) + t4 * 4);
+            const float2 v = unpack2<T>(w);
+            if (see_a) {
+              o[d][0] = fmaf(pa, v.x, o[d][0]);
+              o[d][1] = fmaf(pa, v.y, o[d][1]);
+            }
+            if (see_b) {
+              o[d][2] = fmaf(pb, v.x, o[d][2]);
+              o[d][3] = fmaf(pb, v.y, o[d][3]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[slot]);
+      if (++slot == SLOTS) {
+        slot = 0;
+        parity ^= 1;
+      }
+    }
+    if (!ok) break;
+
+    // ---- merge the warps that took the same rows' keys
+#pragma unroll
+    for (int x = 1; x <= 2; x <<= 1) {
+      l_a += __shfl_xor_sync(0xffffffffu, l_a, x);
+      l_b += __shfl_xor_sync(0xffffffffu, l_b, x);
+    }
+    if constexpr (WK > 1) {
+      if (t4 == 0) {
+        ml_s[warp * 16 + g] = make_float2(m_a, l_a);
+        ml_s[warp * 16 + g + 8] = make_float2(m_b, l_b);
+      }
+      compute_warps_sync();
+      float top_a = -INFINITY, top_b = -INFINITY, sum_a = 0.f, sum_b = 0.f;
+#pragma unroll
+      for (int w = 0; w < WK; ++w) {
+        top_a = fmaxf(top_a, ml_s[(wm * WK + w) * 16 + g].x);
+        top_b = fmaxf(top_b, ml_s[(wm * WK + w) * 16 + g + 8].x);
+      }
+#pragma unroll
+      for (int w = 0; w < WK; ++w) {
+        const float2 xa = ml_s[(wm * WK + w) * 16 + g], xb = ml_s[(wm * WK + w) * 16 + g + 8];
+        sum_a += xa.y * part_weight(xa.x, top_a);
+        sum_b += xb.y * part_weight(xb.x, top_b);
+      }
+      const float fa = part_weight(m_a, top_a), fb = part_weight(m_b, top_b);
+      m_a = top_a;
+      m_b = top_b;
+      l_a = sum_a;
+      l_b = sum_b;
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d) {
+        o[d][0] *= fa;
+        o[d][1] *= fa;
+        o[d][2] *= fb;
+        o[d][3] *= fb;
+      }
+#pragma unroll
+      for (int left = WK / 2; left >= 1; left >>= 1) {
+        float* buf = stage + (wm * (WK / 2) + (wk & (left - 1))) * 16 * DP;
+        if (wk >= left && wk < 2 * left) {
+#pragma unroll
+          for (int d = 0; d < DP / 8; ++d) {
+            *reinterpret_cast<float2*>(buf + g * DP + d * 8 + t4 * 2) = make_float2(o[d][0], o[d][1]);
+            *reinterpret_cast<float2*>(buf + (g + 8) * DP + d * 8 + t4 * 2) = make_float2(o[d][2], o[d][3]);
+          }
+        }
+        compute_warps_sync();
+        if (wk < left) {
+#pragma unroll
+          for (int d = 0; d < DP / 8; ++d) {
+            const float2 xa = *reinterpret_cast<float2*>(buf + g * DP + d * 8 + t4 * 2);
+            const float2 xb = *reinterpret_cast<float2*>(buf + (g + 8) * DP + d * 8 + t4 * 2);
+            o[d][0] += xa.x;
+            o[d][1] += xa.y;
+            o[d][2] += xb.x;
+            o[d][3] += xb.y;
+          }
+        }
+        if (left > 1) compute_warps_sync();
+      }
+    }
+    // ---- output, or a piece for the joining pass
+    const bool begins = off == 0, ends = off + run == at.n;
+    if (wk == 0) {
+      if (begins && ends) {
+        const float ia = inverse_sum(l_a), ib = inverse_sum(l_b);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int r = row0 + g + half * 8;
+          if (r < at.rows) {
+            const long long t = at.s.t0 + r / p.G;
+            const int h = at.hk * p.G + r % p.G;
+            T* dst = static_cast<T*>(p.out) + t * p.os_t + h * p.os_h;
+            const float inv = half ? ib : ia;
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d)
+              if (d * 8 < p.D)
+                *reinterpret_cast<uint32_t*>(dst + d * 8 + t4 * 2) =
+                    pack2<T>(o[d][half * 2] * inv, o[d][half * 2 + 1] * inv);
+            if (p.lse && t4 == 0)
+              p.lse[t * p.Hq + h] = log_sum(half ? m_b : m_a, half ? l_b : l_a);
+          }
+        }
+      } else {
+        const long long slot_row = (2LL * blockIdx.x + (begins ? 1 : 0)) * MR + wm * 16;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float* dst = p.part_o + (slot_row + g + half * 8) * DP;
+#pragma unroll
+          for (int d = 0; d < DP / 8; ++d)
+            *reinterpret_cast<float2*>(dst + d * 8 + t4 * 2) = make_float2(o[d][half * 2], o[d][half * 2 + 1]);
+          if (t4 == 0)
+            p.part_ml[slot_row + g + half * 8] = half ? make_float2(m_b, l_b) : make_float2(m_a, l_a);
+        }
+      }
+    }
+    if (begins && !ends) {  // only ever the run's last row tile
+      wrote_meta = true;
+      if (threadIdx.x == 0) {
+        Entry e;
+        e.pieces = static_cast<int>((u + at.n - 1) / per_block - blockIdx.x) + 1;
+        e.t0 = at.s.t0;
+        e.hk = at.hk;
+        e.row0 = at.rt * MR;
+        e.rows = min(MR, at.rows - at.rt * MR);
+        e.slot0 = 2 * blockIdx.x + 1;
+        e.slot1 = 2 * (blockIdx.x + 1);
+        e.step = 2;
+        *meta = e;
+      }
+    }
+    u += run;
+    off = 0;
+    if (u < u1) at.next();
+  }
+  if (!wrote_meta && threadIdx.x == 0) meta->pieces = 0;
+}
+
+}  // namespace paged
+}  // namespace pkb200

@@ -14,6 +14,7 @@
 // the heads that it visits.
 #pragma once
 
+#include "paged_index.h"
 #include "sm100.cuh"
 
 namespace pkb200 {
@@ -213,19 +214,13 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
   const int* cu = shared ? cu_s : p.cu;
   const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
   const long long token = i / p.row.items;
-  if (token >= p.T || token < cu[0] || token >= cu[p.B]) return;  // rows of no sequence stay
+  if (token >= p.T) return;
   const int item = static_cast<int>(i - token * p.row.items);
-  // the last sequence that starts at or before the token
-  int lo = 0, hi = p.B;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= token) lo = mid;
-    else hi = mid;
-  }
-  const int end = cu[lo + 1];
-  const long long position = static_cast<long long>(__ldg(p.lens + lo)) - end + token;
-  if (token >= end || position < 0) {  // offsets out of order, or a length below the new tokens
-    if (item == 0) atomicCAS(p.err, 0, kErrBadBatch);
+  int seq;
+  long long position;
+  const auto place = paged::place_token(cu, p.B, token, [&](int b) { return __ldg(p.lens + b); }, seq, position);
+  if (place != paged::kPlaced) {  // rows of no sequence stay as they are
+    if (place == paged::kMisplaced && item == 0) atomicCAS(p.err, 0, kErrBadBatch);
     return;
   }
   int u0, u1;
@@ -246,8 +241,10 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p)
     return;
   }
   const long long slot = position / p.page_size;
-  const int page = slot < p.table_width ? __ldg(p.page_table + lo * p.table_stride + slot) : -1;
-  if (page < 0 || page >= p.num_pages) {
+  const int page =
+      slot < p.table_width ? paged::clip_page(__ldg(p.page_table + seq * p.table_stride + slot), p.num_pages)
+                           : p.num_pages;
+  if (page == p.num_pages) {
     if (item == 0) atomicCAS(p.err, 0, kErrBadBatch);
     return;
   }

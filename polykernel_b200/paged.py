@@ -256,3 +256,84 @@ def paged_kv_append(k, v, k_pages, v_pages, page_table, cu_seqlens, seq_lens, in
                 k.data_ptr(), _LL2(*k.stride()[:2]), v.data_ptr(), _LL2(*v.stride()[:2]), *q_args,
                 freq, pairs, float(factor), int(bool(interleaved))), "paged_kv_append")
     return q_out
+
+
+def _aligned(t, name):
+    """16-byte rows: what the copies of attention start on."""
+    if t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
+        raise ValueError(f"{name} must start on 16 bytes, with strides that are multiples of 8 values")
+    return t
+
+
+def _strides(t, make):
+    """Strides without the last axis's; those of axes of one are never taken."""
+    return make(*(s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)))
+
+
+def paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, seq_lens, max_q_len=None, causal=True,
+                    window=None, scale=None, return_lse=False, out=None, lse=None, workspace=None):
+    """Attention of the new tokens q [T, q_heads, dim] over the pages of their
+    sequences (whose new keys are appended first: `paged_kv_append`). Query head h
+    reads key head h // (q_heads / heads). With `causal` a token sees the keys up to
+    its own position, with `window` the last `window` of those. A row that sees no
+    key gives zeros (and -inf). Returns out, or (out, lse) with return_lse, the
+    fp32 [T, q_heads] logarithms of the sums of exponentials; both can be passed in.
+    Rows of no sequence keep what `out` and `lse` held.
+
+    dim and the page size are multiples of 8, dim at most 256. max_q_len, the most
+    new tokens of any sequence, selects kernels and changes no result: pass it for
+    speed (by default 1 for as many tokens as sequences, T otherwise).
+    `workspace`: a uint8 tensor to use instead of a new one, if it is large enough;
+    calls that may overlap need their own."""
+    n = _tokens(q, "q")
+    dev, cache, batch = _paged(k_pages, v_pages, page_table, cu_seqlens, seq_lens, n)
+    dim, hq = cache.dim, q.shape[1]
+    _rows(q, "q", k_pages.dtype, dev, (n, hq, dim))
+    if hq == 0 or hq % cache.heads:
+        raise ValueError(f"{hq} query heads do not divide among {cache.heads} key heads")
+    if dim % 8 or dim > 256:
+        raise ValueError(f"dim must be a multiple of 8 up to 256, got {dim}")
+    if cache.page_size % 8:
+        raise ValueError(f"the page size must be a multiple of 8, got {cache.page_size}")
+    if cache.num_pages == 0:
+        raise ValueError("k_pages has no pages")
+    if n * hq // cache.heads >= 2 ** 31 - 1:
+        raise ValueError("too many tokens for one call")
+    if window is not None and (window < 1 or not causal):
+        raise ValueError("window must be at least 1, and needs causal")
+    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError("scale must be positive and finite")
+    if max_q_len is None:
+        max_q_len = 1 if n <= batch.num_seqs else n
+    elif max_q_len < 0:
+        raise ValueError("max_q_len must not be negative")
+    for t, name in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages")):
+        _aligned(t, name)
+    if out is None:
+        out = torch.empty(n, hq, dim, dtype=q.dtype, device=dev)
+    else:
+        _aligned(_rows(out, "out", q.dtype, dev, (n, hq, dim)), "out")
+    if lse is not None:
+        _tensor(lse, "lse", (torch.float32,), 2, dev)
+        if lse.shape != (n, hq) or not lse.is_contiguous():
+            raise ValueError(f"lse must be contiguous, of shape {(n, hq)}")
+    elif return_lse:
+        lse = torch.empty(n, hq, dtype=torch.float32, device=dev)
+    cache.k_stride, cache.v_stride = _strides(k_pages, _LL3), _strides(v_pages, _LL3)
+    window = min(window or 0, 2 ** 30)
+    max_q_len = min(max_q_len, n)
+
+    def go(stream):
+        nonlocal workspace
+        c, b = ctypes.byref(cache), ctypes.byref(batch)
+        need = lib().pkb200_paged_attention_workspace_size(c, b, hq, max_q_len, window)
+        if workspace is None or workspace.numel() < need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        return lib().pkb200_paged_attention(
+            c, b, q.data_ptr(), _strides(q, _LL2), out.data_ptr(), _strides(out, _LL2),
+            None if lse is None else lse.data_ptr(), hq, max_q_len, int(bool(causal)), window, scale,
+            workspace.data_ptr(), workspace.numel(), stream)
+
+    check(_call(dev, go), "paged_attention")
+    return (out, lse) if return_lse else out

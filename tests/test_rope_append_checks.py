@@ -91,3 +91,53 @@ def test_c_entry_refusals_without_a_device():
             append(num_pages=-1), append(k=None)] == [1] * 15
     assert L.pkb200_paged_kv_append(None, None, p, st, p, st, None, None, None, None, 0, None, 0,
                                     ctypes.c_float(1.0), 0, None) == 1
+
+
+def test_wrong_batches_stay_in_range(tmp_path):
+    """The kernels' index arithmetic over random, mostly wrong, batch descriptions."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = tmp_path / "paged_index_test"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover", "-o", str(exe),
+                    os.path.join(root, "tests", "cpp", "paged_index_test.cpp")], check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert out.returncode == 0 and out.stdout.startswith("ok"), out.stdout + out.stderr
+
+
+def test_attention_c_entry_refusals_without_a_device():
+    from polykernel_b200 import _lib
+    L = _lib.lib()
+    buf = ctypes.create_string_buffer(4096)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    st3, st2 = (ctypes.c_longlong * 3)(64, 64, 64), (ctypes.c_longlong * 2)(64, 64)
+
+    def run(q=p, out=p, hq=1, most=1, causal=1, window=0, scale=1.0, tokens=1, seqs=1, ws=p, q_st=st2,
+            out_st=st2, width=1, **cache):
+        c = dict(k=p, v=p, k_stride=st3, v_stride=st3, num_pages=1, heads=1, page_size=8, dim=64, dtype=0)
+        c.update(cache)
+        c = _lib.PagedCache(**c)
+        b = _lib.PagedBatch(p, p, p, width, width, seqs, tokens)
+        return L.pkb200_paged_attention(ctypes.byref(c), ctypes.byref(b), q, q_st, out, out_st, None, hq, most,
+                                        causal, window, ctypes.c_float(scale), ws, 0, None)
+
+    odd = (ctypes.c_longlong * 2)(64, 60)
+    odd3 = (ctypes.c_longlong * 3)(64, 64, 63)
+    assert [run(tokens=0), run(seqs=0)] == [0, 0]
+    refused = [run(q=None), run(out=None), run(hq=0), run(hq=3, heads=2), run(most=-1), run(window=-1),
+               run(window=5, causal=0), run(scale=0.0), run(scale=-1.0), run(scale=math.nan),
+               run(scale=math.inf), run(tokens=-1), run(dim=60), run(dim=264), run(page_size=12),
+               run(page_size=0), run(num_pages=0), run(dtype=2), run(q=p + 8), run(out=p + 2), run(k=p + 4),
+               run(q_st=odd), run(out_st=odd), run(k_stride=odd3), run(v_stride=odd3), run(k=None),
+               run(tokens=2 ** 30, hq=4, heads=1)]
+    assert refused == [1] * len(refused)
+
+
+def test_attention_python_checks(ops):
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    pool = torch.zeros(1, 1, 8, 64, dtype=torch.bfloat16)
+    i32 = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError):  # CPU tensors
+        ops.paged_attention(q, pool, pool, i32[None], torch.zeros(2, dtype=torch.int32), i32)
+    with pytest.raises(ValueError):
+        ops.paged_attention(q[0], pool, pool, i32[None], i32, i32)
