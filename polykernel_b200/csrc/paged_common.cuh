@@ -96,11 +96,14 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) { return un
 template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) { return unpack_f16x2(v); }
 
-// Whether one of the two values in `w` is infinite or NaN (all exponent bits set).
+// Nonzero if one of the eight values in `w` is infinite or NaN (all exponent bits
+// set): adding one at the lowest exponent bit then carries into the sign bit.
 template <typename T>
-__device__ __forceinline__ bool not_finite2(uint32_t w) {
-  constexpr uint32_t e = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  return (w & e) == e || ((w >> 16) & e) == e;
+__device__ __forceinline__ uint32_t not_finite4(const uint4& w) {
+  constexpr bool half = std::is_same<T, __half>::value;
+  constexpr uint32_t e = half ? 0x7c007c00u : 0x7f807f80u, one = half ? 0x04000400u : 0x00800080u;
+  const uint32_t t = ((w.x & e) + one) | ((w.y & e) + one) | ((w.z & e) + one) | ((w.w & e) + one);
+  return t & 0x80008000u;
 }
 
 // Weight of a part whose maximum is m within a row whose maximum is top.

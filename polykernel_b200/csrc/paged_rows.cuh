@@ -383,8 +383,7 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
           uint4* w = reinterpret_cast<uint4*>(smem + slot * C::SLOT + (c >> 3) * (KT * 128) + key * 128 + (c & 7) * 16);
           if (key0 + key >= at.s.len) *w = make_uint4(0u, 0u, 0u, 0u);
           else {
-            const uint4 v = *w;
-            bad |= not_finite2<T>(v.x) || not_finite2<T>(v.y) || not_finite2<T>(v.z) || not_finite2<T>(v.w);
+            bad |= not_finite4<T>(*w) != 0;
           }
         }
         fence_proxy_async_smem();

@@ -2,22 +2,26 @@
 // prompts and chunks of them (tcgen05, sm_100a).
 //
 // Bound by the tensor cores and, equally, by exp: a pair of 128-row tiles costs
-// 2048 cycles of tensor work per 128-key tile at head width 128, and 2 x 128 x
-// 128 exponentials cost the same at 16 a cycle. One block therefore works on
-// two 128-row tiles (A, B) that share every key tile, and alternates: while the
-// tensor cores form P.V and the next S of one, a warpgroup takes the softmax of
-// the other. Rows are the G heads of consecutive tokens, so a key tile is
-// fetched once for the group.
+// 2048 cycles of tensor work per 128-key tile at head width 128, and their 2 x
+// 128 x 128 exponentials cost the same at 16 a cycle. So a block works on two
+// 128-row tiles (A, B) that share every key tile: while the tensor cores form
+// P.V and the next S of one, a warpgroup takes the softmax of the other; and a
+// part of the exponentials is formed on the FMA pipe. Rows are the G heads of
+// consecutive tokens, so a key tile is fetched once for the group.
 //   warps 0-3, 4-7   softmax of A and of B: thread r owns row r (TMEM lane r),
-//                    reads its 128 scores, and writes P back over them as
-//                    16-bit pairs, the A operand of P.V.
-//   warps 8-11       correction: rescale O in TMEM when a row's maximum moved
-//                    by more than 2^8 (P stays below 2^8, the sums share the
-//                    stale maximum, so the quotient is exact), and the epilogue.
-//   warp 12          TMA: Q once, key and value pages into one ring.
-//   warp 13          MMA issuer and TMEM owner.
-//   warps 14, 15     clear value rows past the end of a sequence and look for
+//                    reads its 128 scores, writes P back over them as 16-bit
+//                    pairs (the A operand of P.V), rescales O in TMEM when the
+//                    row's maximum moved by more than 2^8 (P stays below 2^8 and
+//                    the sums share the stale maximum, so the quotient is
+//                    exact), and writes the output.
+//   warps 8-11       clear value rows past the end of a sequence and look for
 //                    values that are not finite in tiles that some row masks.
+//   warp 12          TMA: Q, and key and value pages into one ring.
+//   warp 13          MMA issue, and owner of TMEM.
+//   warp 14          work: blocks stay resident and take over the work of blocks
+//                    that have not been launched yet (cluster launch control),
+//                    in the grid's order, one item ahead of the other warps.
+//   (warp 15 completes a warpgroup.)
 // TMEM: S/P of A [0,128), of B [128,256), O of A [256,384), of B [384,512).
 //
 // P is rounded once to the inputs' type (bf16: 2^-9 relative, fp16: 2^-12),
@@ -25,7 +29,7 @@
 // are independent, so the output's stays at the level of its own rounding.
 // The row sums are of the unrounded P, in fp32.
 //
-// With few row tiles over a long cache, `splits` blocks share a tile's keys and
+// With few row tiles over a long cache, `splits` items share a tile's keys and
 // paged_join_kernel adds their pieces up.
 #pragma once
 
@@ -42,19 +46,110 @@ struct TilesCfg {
   static constexpr int TILE = 128 * DP * 2;  // one 128-row tile of Q, K or V
   static constexpr int STAGES = DP == 128 ? 4 : 8;
   static constexpr int OFF_KV = 2 * TILE;
-  static constexpr int OFF_ALPHA = OFF_KV + STAGES * TILE;  // float[2][128]
-  static constexpr int OFF_ML = OFF_ALPHA + 2 * 128 * 4;    // float2[2][128]
-  static constexpr int OFF_BAR = OFF_ML + 2 * 128 * 8;
-  static constexpr int SMEM = OFF_BAR + 512 + 1024;
-  static constexpr int kRegsSoftmax = 192, kRegsCorrection = 80, kRegsControl = 48;
-  static_assert(2 * kRegsSoftmax + kRegsCorrection + kRegsControl == 4 * 128, "launch: 512 x 128");
+  static constexpr int OFF_OUT = OFF_KV + STAGES * TILE;  // 4 KB per softmax warp
+  static constexpr int OFF_WORK = OFF_OUT + 8 * 4096;     // TileWork[2]
+  static constexpr int OFF_BAR = OFF_WORK + 2 * 64;
+  static constexpr int kBarBytes = 512;
+  static constexpr int SMEM = OFF_BAR + kBarBytes + 1024;
+  static constexpr int kRegsSoftmax = 176, kRegsValues = 80, kRegsControl = 80;
+  static_assert(2 * kRegsSoftmax + kRegsValues + kRegsControl == 4 * 128, "launch: 512 x 128");
+  static_assert(SMEM <= 232448, "shared memory of an SM");
 };
 constexpr float kStaleMax = 8.f;  // log2 units a row's maximum may lag behind
+
+// One item of work, as the work warp hands it to the others.
+struct alignas(64) TileWork {
+  int b;              // sequence; -1: no more items
+  Seq s;
+  int first, count;   // tokens of both tiles
+  int hk, tile0, nt;  // key head, key tiles [tile0, tile0 + nt)
+  int pieces, slot;   // pieces of these rows' keys, and where this one goes
+  int all_lo, all_hi; // keys that every row sees
+  int by_hand;        // values of masked keys are not finite
+};
+static_assert(sizeof(TileWork) == 64, "");
+
+// 2^x of a pair on the FMA and integer pipes, for x >= -126; values from -127
+// down (and -inf) give 0. The SFU takes 8 cycles for a warp's ex2, which would
+// bound the softmax alone. x = n + f with n whole and |f| <= 1/2 (adding 1.5 *
+// 2^23 rounds to whole numbers and leaves n in the low bits); 2^f = 1 + f (c1 +
+// ...), the degree-4 polynomial of that form with the least relative error on
+// the interval (iterated weighted least squares: 2.9e-6, below the rounding of
+// P); n goes into the exponent. NaN is not carried through.
+__device__ __forceinline__ void exp2_pair(uint64_t x2, float& e0, float& e1) {
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23
+  constexpr float c1 = 0.69312418f, c2 = 0.24024099f, c3 = 0.055906426f, c4 = 0.009582853f;
+  float x0, x1;
+  f2_unpack(x2, x0, x1);
+  x2 = f2_pack(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
+  const uint64_t t2 = f2_add(x2, f2_pack(kRound, kRound));
+  const uint64_t f2 = f2_sub(x2, f2_sub(t2, f2_pack(kRound, kRound)));
+  uint64_t p2 = f2_fma(f2_pack(c4, c4), f2, f2_pack(c3, c3));
+  p2 = f2_fma(p2, f2, f2_pack(c2, c2));
+  p2 = f2_fma(p2, f2, f2_pack(c1, c1));
+  p2 = f2_fma(p2, f2, f2_pack(1.f, 1.f));
+  float t0, t1, p0, p1;
+  f2_unpack(t2, t0, t1);
+  f2_unpack(p2, p0, p1);
+  e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+  e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
+
+// max of three that is NaN if one of them is.
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Asks for the work of a block that has not been launched yet; the answer, 16
+// bytes at `answer`, completes `bar`.
+__device__ __forceinline__ void take_block_async(void* answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+          smem_u32(answer)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+// The index of the block taken over, -1 if there is none left.
+__device__ __forceinline__ int taken_block(const void* answer) {
+  int got;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 r, [%1];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "mov.s32 %0, -1;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n\t}"
+      : "=r"(got)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return got;
+}
 
 template <typename T>
 constexpr uint32_t mma_desc(int n, bool b_mn_major) {
   return std::is_same<T, __half>::value ? make_idesc_f16(128, n, false, b_mn_major)
                                         : make_idesc_bf16(128, n, false, b_mn_major);
+}
+
+// The MMAs of one tile, issued warp-wide (tc_mma_f16_warp); descriptors advance by
+// constants. S [128 x 128] = Q K^T: 16 columns of the head per MMA, 32 bytes
+// within a 128-byte row, 16 KB between 64-column halves.
+template <typename T, int DP>
+__device__ __forceinline__ void issue_s(uint32_t s_tmem, uint64_t q_desc, uint64_t k_desc) {
+#pragma unroll
+  for (int kk = 0; kk < DP / 16; ++kk) {
+    const uint64_t off = (kk >> 2) * 1024 + (kk & 3) * 2;
+    tc_mma_f16_warp(s_tmem, q_desc + off, k_desc + off, mma_desc<T>(128, false), kk != 0);
+  }
+}
+// O [128 x DP] (+)= P V for the keys [16 FROM, 16 TO): 8 TMEM columns and 2 KB of V each.
+template <typename T, int DP, int FROM, int TO>
+__device__ __forceinline__ void issue_pv(uint32_t o_tmem, uint32_t p_tmem, uint64_t v_desc, uint32_t add) {
+#pragma unroll
+  for (int kk = FROM; kk < TO; ++kk)
+    tc_mma_f16_tmem_a_warp(o_tmem, p_tmem + kk * 8, v_desc + kk * 128, mma_desc<T>(DP, true),
+                           kk == FROM ? add : 1u);
 }
 
 // One row's attention over the keys [k0, k1) that it sees, by one warp, in fp32
@@ -124,120 +219,53 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  float* alpha_s = reinterpret_cast<float*>(smem + C::OFF_ALPHA);
-  float2* ml_s = reinterpret_cast<float2*>(smem + C::OFF_ML);
+  TileWork* work = reinterpret_cast<TileWork*>(smem + C::OFF_WORK);  // [2]
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);  // [STAGES]
   uint64_t* empty = full + STAGES;                                  // [STAGES]
-  uint64_t* q_full = empty + STAGES;
-  uint64_t* s_full = q_full + 1;       // [2] S of the tile is in TMEM
-  uint64_t* alpha_full = s_full + 2;   // [2] its rescale factors are in alpha_s
-  uint64_t* p_ready = alpha_full + 2;  // [2] P is in TMEM and O is rescaled
-  uint64_t* o_done = p_ready + 2;      // [2] P.V is added to O
-  uint64_t* ml_full = o_done + 2;      // [2] final maxima and sums are in ml_s
   // A masked value tile is on its way into that stage (the stage's earlier
   // phases are over, so that its `full` can be waited on by parity), and its
   // values are cleared and looked at. Per stage: several may be under way.
-  uint64_t* v_look = ml_full + 2;      // [STAGES]
+  uint64_t* v_look = empty + STAGES;   // [STAGES]
   uint64_t* v_fixed = v_look + STAGES; // [STAGES]
-  long long* scan = reinterpret_cast<long long*>(v_fixed + STAGES);  // [16]
-  int* found = reinterpret_cast<int*>(scan + 16);               // sequence, tile
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(found + 2);
+  uint64_t* q_full = v_fixed + STAGES;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;      // [2] S of the tile is in TMEM
+  uint64_t* p_ready = s_full + 2;      // [2] P of 96 keys is in TMEM and O is rescaled
+  uint64_t* p_rest = p_ready + 2;      // [2] P of the other 32
+  uint64_t* o_full = p_rest + 2;       // [2] the item's last P.V is added to O
+  uint64_t* work_full = o_full + 2;    // [2]
+  uint64_t* work_empty = work_full + 2;  // [2]
+  uint64_t* taken = work_empty + 2;    // the answer about the next block is there
+  uint64_t* ask = taken + 1;           // the item's loads are nearly all issued
+  void* answer = taken + 2;            // 16 bytes, 16-byte aligned
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* by_hand = abort_flag + 1;
-  static_assert((4 * STAGES + 11) * 8 + 16 * 8 + 5 * 4 <= 512, "barrier area");
+  static_assert((4 * STAGES + 18) * 8 + 8 <= C::kBarBytes, "barrier area");
+  static_assert((4 * STAGES + 16) % 2 == 0, "the answer is 16-byte aligned");
   const int warp = warp_id(), lane = lane_id();
+  const int tok = 128 / p.G;  // tokens of a 128-row tile
 
   grid_launch_dependents();
-  // Block order: row tiles fastest, the longest first, then key heads, then
-  // pieces of the keys, so that blocks which run together share keys in L2.
-  const int tile = static_cast<int>(blockIdx.x) % p.tiles;
-  const int hk = static_cast<int>(blockIdx.x) / p.tiles % p.Hkv;
-  const int split = static_cast<int>(blockIdx.x) / p.tiles / p.Hkv;
-  const int entry = hk * p.tiles + tile;
-  Entry* const meta = reinterpret_cast<Entry*>(p.meta) + entry;
-  const int tok = 128 / p.G;  // tokens of a 128-row tile
-  auto tiles_of = [&](const Seq& s) {
-    const int rows = s.nq * p.G;
-    return rows >= p.min_rows && rows <= p.max_rows ? (s.nq + 2 * tok - 1) / (2 * tok) : 0;
-  };
-  {
-    const int each = (p.B + C::kThreads - 1) / C::kThreads;
-    const int b0 = static_cast<int>(threadIdx.x) * each, b1 = min(p.B, b0 + each);
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += tiles_of(load_seq(p, b, true));
-    long long total;
-    const long long before = block_prefix<C::kThreads>(mine, scan, total);
-    if (tile >= total) {
-      if (p.splits > 1 && split == 0 && threadIdx.x == 0) meta->pieces = 0;
-      return;
-    }
-    if (tile >= before && tile < before + mine) {
-      int at = static_cast<int>(before);
-      for (int b = b0;; ++b) {
-        const int n = tiles_of(load_seq(p, b));
-        if (tile < at + n) {
-          found[0] = b;
-          found[1] = n - 1 - (tile - at);
-          break;
-        }
-        at += n;
-      }
-    }
-    __syncthreads();
-  }
-  const int b = found[0];
-  const Seq s = load_seq(p, b);
-  const int first = found[1] * 2 * tok;                  // first token
-  const int count = min(2 * tok, s.nq - first);          // tokens of both tiles
-  const int rows = count * p.G;
-  const bool two = count > tok;
-  int tile0, tile1;
-  int pieces;
-  {
-    int base;
-    const int n = key_tiles<KT>(p, s, first, first + count - 1, base);
-    pieces = min(p.splits, max(1, n / p.min_units));
-    if (split >= pieces) return;
-    tile0 = base + static_cast<int>(static_cast<long long>(n) * split / pieces);
-    tile1 = base + static_cast<int>(static_cast<long long>(n) * (split + 1) / pieces);
-  }
-  const int nt = tile1 - tile0;
-  if (split == 0 && p.splits > 1 && threadIdx.x == 0) {
-    Entry e;
-    e.pieces = pieces > 1 ? pieces : 0;
-    e.t0 = s.t0;
-    e.hk = hk;
-    e.row0 = first * p.G;
-    e.rows = rows;
-    e.slot0 = entry * p.splits;
-    e.slot1 = e.slot0 + 1;
-    e.step = 1;
-    *meta = e;
-  }
-  // keys that every row of the block sees
-  const int all_hi = key_hi(p, s, first), all_lo = key_lo(p, s, first + count - 1);
-  auto masked = [&](int j) {
-    const int key0 = (tile0 + j) * KT;
-    return key0 + KT > all_hi || key0 < all_lo;
-  };
-
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
       mbar_init(&v_look[i], 1);
-      mbar_init(&v_fixed[i], 64);
+      mbar_init(&v_fixed[i], 128);
     }
     mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int x = 0; x < 2; ++x) {
       mbar_init(&s_full[x], 1);
-      mbar_init(&alpha_full[x], 128);
-      mbar_init(&p_ready[x], 256);
-      mbar_init(&o_done[x], 1);
-      mbar_init(&ml_full[x], 128);
+      mbar_init(&p_ready[x], 128);
+      mbar_init(&p_rest[x], 128);
+      mbar_init(&o_full[x], 1);
+      mbar_init(&work_full[x], 1);
+      mbar_init(&work_empty[x], 14);
     }
+    mbar_init(taken, 1);
+    mbar_init(ask, 1);
     *abort_flag = 0;
-    *by_hand = 0;
     fence_barrier_init();
   }
   if (warp == 13) {
@@ -249,148 +277,281 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  // Whole-warp wait; false if the kernel is to be given up: another role did,
+  // or the limit ran out (`late` then tells that this warp is the first). The
+  // limit leaves room for rows that are formed one by one.
+  constexpr long long kLimit = 4 * kSpinLimitCycles;
+  bool ok = true, late = false;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    const long long t0 = clock64();
+    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+      if (*abort_flag) return false;
+      if (clock64() - t0 > kLimit) {
+        late = true;
+        *abort_flag = 1;
+        return false;
+      }
+    }
+    return true;
+  };
+  // For what is in flight into this block's memory when the kernel is given up.
+  auto wait_late = [&](uint64_t* bar, uint32_t parity) {
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity) && clock64() - t0 < kSpinLimitCycles) {}
+    return false;
+  };
+  // The next item for this warp (`item` counts them); false at the end.
+  int item = 0;
+  auto next_work = [&] {
+    ok = wait(&work_full[item & 1], (item >> 1) & 1);
+    return ok && work[item & 1].b >= 0;
+  };
+  auto release_work = [&] {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&work_empty[item & 1]);
+    ++item;
+  };
+  auto masked = [&](const TileWork& w, int j) {
+    const int key0 = (w.tile0 + j) * KT;
+    return key0 + KT > w.all_hi || key0 < w.all_lo;
+  };
+
   if (warp >= 12) {
     setmaxnreg_dec<C::kRegsControl>();
     if (warp == 12) {
       // ------------------------------------------------------------ fetch --
       if (lane == 0) {
-        mbar_arrive_expect_tx(q_full, (two ? 2 : 1) * C::HALVES * tok * p.G * 128);
-        for (int x = 0; x < (two ? 2 : 1); ++x)
-          for (int c = 0; c < C::HALVES; ++c)
-            tma_load_3d(smem + x * C::TILE + c * (128 * 128), &map_q, q_full, c * 64, hk * p.G,
-                        s.t0 + first + x * tok);
+        tma_prefetch_desc(&map_q);
+        tma_prefetch_desc(&map_k);
+        tma_prefetch_desc(&map_v);
       }
-      __syncwarp();
       const int boxes = KT / p.box;
       const int col = lane / boxes, bx = lane - col * boxes;
       const bool mine = col < C::HALVES;
-      auto lookup = [&](int j) {
-        const int key = (tile0 + j) * KT + bx * p.box;
-        return mine && key < s.len ? page_of(p, b, key) : -1;
-      };
       int stage = 0, issued = 0;
       uint32_t parity = 1;
-      bool ok = true;
-      int page = lookup(0);
-      for (int j = 0; j < nt && ok; ++j) {
-        const int next = j + 1 < nt ? lookup(j + 1) : -1;
-        const int row = ((tile0 + j) * KT + bx * p.box) % p.page_size;
-        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, page >= 0)) * p.box * 128;
+      while (ok && next_work()) {
+        const TileWork w = work[item & 1];
+        const bool two = w.count > tok;
+        auto lookup = [&](int j) {
+          const int key = (w.tile0 + j) * KT + bx * p.box;
+          return mine && key < w.s.len ? page_of(p, w.b, key) : -1;
+        };
+        int page = lookup(0);
+        for (int j = 0; j < w.nt && ok; ++j) {
+          if (j == max(0, w.nt - 3) && lane == 0) mbar_arrive(ask);
+          const int next = j + 1 < w.nt ? lookup(j + 1) : -1;
+          const int row = ((w.tile0 + j) * KT + bx * p.box) % p.page_size;
+          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, page >= 0)) * p.box * 128;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          ok = ok && __all_sync(0xffffffffu, mbar_wait(&empty[stage], parity, p.err, abort_flag,
-                                                       kErrTimeoutProducer));
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&full[stage], bytes);
-          __syncwarp();
-          if (page >= 0)
-            tma_load_4d(smem + C::OFF_KV + stage * C::TILE + col * (KT * 128) + bx * p.box * 128,
-                        kv ? &map_v : &map_k, &full[stage], col * 64, row, hk, page);
-          if (kv && lane == 0 && masked(j)) mbar_arrive(&v_look[stage]);
-          ++issued;
-          if (++stage == STAGES) {
-            stage = 0;
-            parity ^= 1;
+          for (int kv = 0; kv < 2; ++kv) {
+            ok = ok && wait(&empty[stage], parity);
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&full[stage], bytes);
+            __syncwarp();
+            if (page >= 0)
+              tma_load_4d(smem + C::OFF_KV + stage * C::TILE + col * (KT * 128) + bx * p.box * 128,
+                          kv ? &map_v : &map_k, &full[stage], col * 64, row, w.hk, page);
+            if (kv && lane == 0 && masked(w, j)) mbar_arrive(&v_look[stage]);
+            ++issued;
+            if (++stage == STAGES) {
+              stage = 0;
+              parity ^= 1;
+            }
+            if (j == 0 && kv == 0) {  // Q, once the last item's scores are formed
+              ok = wait(q_empty, (item & 1) ^ 1);
+              if (!ok) break;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(q_full, (two ? 2 : 1) * C::HALVES * tok * p.G * 128);
+                for (int x = 0; x < (two ? 2 : 1); ++x)
+                  for (int c = 0; c < C::HALVES; ++c)
+                    tma_load_3d(smem + x * C::TILE + c * (128 * 128), &map_q, q_full, c * 64,
+                                w.hk * p.G, w.s.t0 + w.first + x * tok);
+              }
+              __syncwarp();
+            }
           }
+          page = next;
         }
-        page = next;
+        if (ok) release_work();
       }
-      if (!ok || *abort_flag) {  // do not leave while copies into this block's memory are in flight
-        const long long t0 = clock64();
-        while (!mbar_try_wait(q_full, 0) && clock64() - t0 < kSpinLimitCycles) {}
-        for (int i = max(0, issued - STAGES); i < issued; ++i)
-          while (!mbar_try_wait(&full[i % STAGES], (i / STAGES) & 1) && clock64() - t0 < kSpinLimitCycles) {}
+      if (*abort_flag) {
+        wait_late(q_full, item & 1);
+        for (int i = max(0, issued - STAGES); i < issued; ++i) wait_late(&full[i % STAGES], (i / STAGES) & 1);
       }
     } else if (warp == 13) {
-      // ------------------------------------------------------- MMA issuer --
-      // The whole warp runs the loop; one elected lane issues.
-      constexpr uint32_t desc_s = mma_desc<T>(KT, false), desc_o = mma_desc<T>(DP, true);
-      const uint32_t q_addr = smem_u32(smem), kv_addr = smem_u32(smem + C::OFF_KV);
-      auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err, abort_flag, kErrTimeoutMma));
-      };
-      auto issue_s = [&](int x, int j) {
-        const uint32_t k_addr = kv_addr + (2 * j % STAGES) * C::TILE;
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint32_t at = (kk >> 2) * (128 * 128) + (kk & 3) * 32;
-          tc_mma_f16_warp(tmem + x * 128, make_sw128_desc(q_addr + x * C::TILE + at, 16, 1024),
-                          make_sw128_desc(k_addr + at, 16, 1024), desc_s, kk != 0);
-        }
-        tc_commit_warp(&s_full[x]);
-      };
-      auto issue_pv = [&](int x, int j) {
-        const uint32_t v_addr = kv_addr + ((2 * j + 1) % STAGES) * C::TILE;
-#pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk)
-          tc_mma_f16_tmem_a_warp(tmem + 256 + x * 128, tmem + x * 128 + kk * 8,
-                                 make_sw128_desc(v_addr + kk * 2048, KT * 128, 1024), desc_o,
-                                 (j != 0 || kk != 0));
-        tc_commit_warp(&o_done[x]);
-      };
-      const int last = two ? 1 : 0;
-      bool ok = wait(q_full, 0) && wait(&full[0], 0);
-      if (ok) {
-        tc_fence_after();
-        for (int x = 0; x <= last; ++x) issue_s(x, 0);
-        tc_commit_warp(&empty[0]);
-      }
+      // -------------------------------------------------------- MMA issue --
+      // The whole warp runs the loop; one elected lane issues. One warp serves both tiles
+      // in turn: with a warp for each, their MMAs interleave in the tensor pipe,
+      // both softmaxes wait at once, and the pipe runs dry. The loop is kept
+      // short (one place for S, one for P.V): all roles share the instruction
+      // cache with the softmax, whose unrolled loop alone is some 25 KB.
+      const uint64_t q_desc = make_sw128_desc(smem_u32(smem), 16, 1024);
+      const uint64_t k_desc = make_sw128_desc(smem_u32(smem + C::OFF_KV), 16, 1024);
+      const uint64_t v_desc = make_sw128_desc(smem_u32(smem + C::OFF_KV), KT * 128, 1024);
+      uint32_t place = 0;  // of the item's first key tile in the ring
       uint32_t fixed = 0;  // phases of v_fixed, a bit per stage
-      for (int j = 0; j < nt && ok; ++j) {
-        const int cv = 2 * j + 1, ck = 2 * j + 2;  // places of V(j) and K(j + 1) in the ring
-        ok = wait(&full[cv % STAGES], (cv / STAGES) & 1);
-        if (ok && masked(j)) {
-          ok = wait(&v_fixed[cv % STAGES], (fixed >> (cv % STAGES)) & 1);
-          fixed ^= 1u << (cv % STAGES);
-        }
-        for (int x = 0; x <= last && ok; ++x) {
-          ok = wait(&p_ready[x], j & 1);
-          if (!ok) break;
-          tc_fence_after();
-          issue_pv(x, j);
-          if (x == last) tc_commit_warp(&empty[cv % STAGES]);
-          if (j + 1 < nt) {
-            // S(j + 1) overwrites P(j), which the P.V just issued reads first:
-            // MMAs run in the order of their issue.
-            if (x == 0) {
-              ok = wait(&full[ck % STAGES], (ck / STAGES) & 1);
+      uint32_t done = 0;   // phases of p_ready, a bit per tile
+      while (ok && next_work()) {
+        const TileWork& w = work[item & 1];
+        const int nt = w.nt, tile0 = w.tile0, all_lo = w.all_lo, all_hi = w.all_hi;
+        const int last = w.count > tok ? 1 : 0;
+        for (int j = -1; j < nt && ok; ++j) {  // P.V(j), then S(j + 1)
+          const uint32_t cv = place + 2 * j + 1, ck = cv + 1;
+          const uint32_t sv = cv % STAGES, sk = ck % STAGES;
+          const bool more = j + 1 < nt;
+          if (j >= 0) {
+            const int key0 = (tile0 + j) * KT;
+            ok = wait(&full[sv], (cv / STAGES) & 1);
+            if (ok && (key0 + KT > all_hi || key0 < all_lo)) {
+              ok = wait(&v_fixed[sv], (fixed >> sv) & 1);
+              fixed ^= 1u << sv;
+            }
+          }
+#pragma unroll 1
+          for (int x = 0; x <= last && ok; ++x) {
+            const uint32_t s_tmem = tmem + x * 128;
+            if (j >= 0) {
+              const uint32_t o_tmem = tmem + 256 + x * 128;
+              const uint64_t vd = v_desc + sv * (C::TILE >> 4);
+              ok = wait(&p_ready[x], (done >> x) & 1);
               if (!ok) break;
               tc_fence_after();
+              issue_pv<T, DP, 0, 6>(o_tmem, s_tmem, vd, j != 0);
+              ok = wait(&p_rest[x], (done >> x) & 1);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv<T, DP, 6, 8>(o_tmem, s_tmem, vd, 1);
+              done ^= 1u << x;
+              if (x == last) tc_commit_warp(&empty[sv]);
+              if (!more) tc_commit_warp(&o_full[x]);
             }
-            issue_s(x, j + 1);
-            if (x == last) tc_commit_warp(&empty[ck % STAGES]);
+            if (more) {
+              // S(j + 1) overwrites P(j), which the P.V just issued reads first:
+              // MMAs run in the order of their issue.
+              if (x == 0) {
+                ok = wait(&full[sk], (ck / STAGES) & 1);
+                if (ok && j < 0) ok = wait(q_full, item & 1);
+                if (!ok) break;
+                tc_fence_after();
+              }
+              issue_s<T, DP>(s_tmem, q_desc + x * (C::TILE >> 4), k_desc + sk * (C::TILE >> 4));
+              tc_commit_warp(&s_full[x]);
+              if (x == last) {
+                tc_commit_warp(&empty[sk]);
+                if (j + 2 == nt) tc_commit_warp(q_empty);
+              }
+            }
           }
         }
+        place += 2 * nt;
+        if (ok) release_work();
       }
-    } else {
-      // ------------------------------------------ values of masked tiles --
-      const int t = static_cast<int>(threadIdx.x) - 14 * 32;
-      uint32_t looked = 0;  // phases of v_look, a bit per stage
-      for (int j = 0; j < nt; ++j) {
-        if (!masked(j)) continue;
-        const int cv = 2 * j + 1, st = cv % STAGES;
-        if (!__all_sync(0xffffffffu, mbar_wait(&v_look[st], (looked >> st) & 1, p.err, abort_flag,
-                                               kErrTimeoutConvert) &&
-                                         mbar_wait(&full[st], (cv / STAGES) & 1, p.err, abort_flag,
-                                                   kErrTimeoutConvert)))
-          break;
-        looked ^= 1u << st;
-        uint8_t* v = smem + C::OFF_KV + st * C::TILE;
-        const int key0 = (tile0 + j) * KT;
-        bool bad = false;
-#pragma unroll 4
-        for (int i = t; i < KT * C::HALVES * 8; i += 64) {
-          const int key = (i >> 3) % KT;
-          uint4* w = reinterpret_cast<uint4*>(v + i * 16);
-          if (key0 + key >= s.len) *w = make_uint4(0u, 0u, 0u, 0u);
-          else {
-            const uint4 u = *w;
-            bad |= not_finite2<T>(u.x) || not_finite2<T>(u.y) || not_finite2<T>(u.z) || not_finite2<T>(u.w);
+    } else if (warp == 14) {
+      // ------------------------------------------------------------- work --
+      // Items in block order: row tiles fastest, a sequence's longest first,
+      // then key heads, then pieces of the keys, so that items which run
+      // together share keys in L2.
+      int block = blockIdx.x;
+      bool report = true;
+      int asked = 0;
+      for (;; ++asked) {
+        const int tile = block % p.tiles, hk = block / p.tiles % p.Hkv, split = block / p.tiles / p.Hkv;
+        const int entry = hk * p.tiles + tile;
+        // the sequence that has this row tile, 32 sequences at a time
+        TileWork w;
+        w.b = -1;
+        Seq s;
+        int n_of = 0, before = 0;
+        for (int b0 = 0; b0 < p.B; b0 += 32) {
+          int n = 0;
+          if (b0 + lane < p.B) {
+            s = load_seq(p, b0 + lane, report);
+            const int rows = s.nq * p.G;
+            n = rows >= p.min_rows && rows <= p.max_rows ? (s.nq + 2 * tok - 1) / (2 * tok) : 0;
           }
+          int upto = n;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+          }
+          const uint32_t hit = __ballot_sync(0xffffffffu, before + upto > tile);
+          if (hit) {
+            const int from = __ffs(hit) - 1;
+            w.b = b0 + from;
+            n_of = __shfl_sync(0xffffffffu, n, from);
+            before = __shfl_sync(0xffffffffu, before + upto - n, from);
+            break;
+          }
+          before += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (bad) *by_hand = 1;
-        fence_proxy_async_smem();
-        mbar_arrive(&v_fixed[st]);
+        bool live = w.b >= 0;
+        w.pieces = 0;
+        if (live) {
+          s = load_seq(p, w.b);
+          w.s = s;
+          w.first = (n_of - 1 - (tile - before)) * 2 * tok;
+          w.count = min(2 * tok, s.nq - w.first);
+          w.hk = hk;
+          int base;
+          const int n = key_tiles<KT>(p, s, w.first, w.first + w.count - 1, base);
+          w.pieces = min(p.splits, max(1, n / p.min_units));
+          w.tile0 = base + static_cast<int>(static_cast<long long>(n) * split / w.pieces);
+          w.nt = base + static_cast<int>(static_cast<long long>(n) * (split + 1) / w.pieces) - w.tile0;
+          w.slot = entry * p.splits + split;
+          w.all_hi = key_hi(p, s, w.first);
+          w.all_lo = key_lo(p, s, w.first + w.count - 1);
+          w.by_hand = 0;
+          live = split < w.pieces;
+        }
+        if (split == 0 && p.splits > 1 && lane == 0) {
+          Entry e = {};
+          if (live && w.pieces > 1) {
+            e.pieces = w.pieces;
+            e.t0 = s.t0;
+            e.hk = hk;
+            e.row0 = w.first * p.G;
+            e.rows = w.count * p.G;
+            e.slot0 = entry * p.splits;
+            e.slot1 = e.slot0 + 1;
+            e.step = 1;
+          }
+          reinterpret_cast<Entry*>(p.meta)[entry] = e;
+        }
+        if (live) {
+          if (!wait(&work_empty[item & 1], ((item >> 1) & 1) ^ 1)) break;
+          if (lane == 0) {
+            work[item & 1] = w;
+            mbar_arrive(&work_full[item & 1]);
+          }
+          __syncwarp();
+          ++item;
+        }
+        report = false;
+        // The next block is asked for when this item's loads are nearly done and
+        // not before: what a block holds back, an idle one cannot take.
+        if (live && !wait(ask, (item - 1) & 1)) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(taken, 16);
+          take_block_async(answer, taken);
+        }
+        __syncwarp();
+        // (waited for to the limit even when the kernel is given up: the answer
+        // is written into this block's memory)
+        const bool answered = wait(taken, asked & 1) || wait_late(taken, asked & 1);
+        block = answered ? taken_block(answer) : -1;
+        fence_proxy_async_smem();  // before the next answer overwrites this one
+        __syncwarp();
+        if (block < 0) {
+          if (answered && wait(&work_empty[item & 1], ((item >> 1) & 1) ^ 1) && lane == 0) {
+            work[item & 1].b = -1;
+            mbar_arrive(&work_full[item & 1]);
+          }
+          __syncwarp();
+          break;
+        }
       }
     }
   } else if (warp < 8) {
@@ -398,187 +559,250 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
     setmaxnreg_inc<C::kRegsSoftmax>();
     const int x = warp >> 2;
     const int r = static_cast<int>(threadIdx.x) & 127;
-    // rows past the tile's last one repeat it; nobody reads them
-    const int i = first + min(x * tok + r / p.G, count - 1);
-    const int hi = key_hi(p, s, i), lo = key_lo(p, s, i);
-    const uint32_t sp = tmem + x * 128 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < nt && (x == 0 || two); ++j) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[x], j & 1, p.err, abort_flag, kErrTimeoutSoftmax)))
-        break;
-      tc_fence_after();
-      uint32_t sv[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(sp + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[c * 32]));
-      tmem_ld_wait();
-      const int key0 = (tile0 + j) * KT;
-      if (__any_sync(0xffffffffu, key0 + KT > hi || key0 < lo)) {
-#pragma unroll
-        for (int c = 0; c < 128; ++c)
-          if (key0 + c >= hi || key0 + c < lo) sv[c] = __float_as_uint(-INFINITY);
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + x * 128 + lanes, o_tmem = tmem + 256 + x * 128 + lanes;
+    uint8_t* stage = smem + C::OFF_OUT + warp * 4096;
+    uint32_t tiles = 0, outputs = 0;
+    while (ok && next_work()) {
+      const TileWork& w = work[item & 1];
+      const int nt = w.nt, tile0 = w.tile0;
+      if (x == 1 && w.count <= tok) {
+        release_work();
+        continue;
       }
-      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      // rows past the tile's last one repeat it; nobody reads them
+      const int i = w.first + min(x * tok + r / p.G, w.count - 1);
+      const int hi = key_hi(p, w.s, i), lo = key_lo(p, w.s, i);
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < nt; ++j, ++tiles) {
+        ok = wait(&s_full[x], tiles & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const int key0 = (tile0 + j) * KT;
+        const int begin = lo - key0, end = hi - key0;  // columns that this row sees
+        const bool hides = __any_sync(0xffffffffu, end < KT || begin > 0);
+        uint32_t sv[128];
 #pragma unroll
-      for (int k = 0; k < 64; ++k)
-        mx4[k & 3] = fmax3(mx4[k & 3], __uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1]));
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
-      float alpha = 1.f;
-      if (mx > m + kStaleMax || (m == -INFINITY && mx > -INFINITY)) {
-        alpha = part_weight(m, mx);
-        l *= alpha;
-        m = mx;
-      }
-      alpha_s[x * 128 + r] = alpha;
-      mbar_arrive(&alpha_full[x]);
-      const float neg = m == -INFINITY ? 0.f : -m;
-      const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), ng2 = f2_pack(neg, neg);
-      uint64_t sum2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&sv[c * 32]));
+        tmem_ld_wait();
+        if (hides) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const int at = c * 32 + 2 * k;
-          float e0, e1;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])), sc2, ng2), e0, e1);
-          e0 = fast_exp2(e0);
-          e1 = fast_exp2(e1);
-          sum2[k & 1] = f2_add(sum2[k & 1], f2_pack(e0, e1));
-          pk[k] = pack2<T>(e0, e1);
+          for (int c = 0; c < 128; ++c)
+            if (c < begin || c >= end) sv[c] = __float_as_uint(-INFINITY);
         }
-        tmem_st16(sp + c * 16, pk);
-      }
-      {
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < 64; ++k)
+          mx4[k & 3] = fmax3_nan(mx4[k & 3], __uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1]));
+        const float mx = fmax3_nan(fmax3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * p.scale_log2;
+        float alpha = 1.f;
+        if (mx > m + kStaleMax || (m == -INFINITY && mx > -INFINITY)) {
+          alpha = part_weight(m, mx);
+          l *= alpha;
+          m = mx;
+        }
+        // A NaN or +inf score makes its row NaN, as inf - inf does; it goes
+        // into the sum here, since exp2_pair would lose it.
+        if (!(mx < INFINITY)) l = NAN;
+        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+          // (P.V of the tile before this one precedes S in the tensor pipe)
+#pragma unroll
+          for (int c = 0; c < DP / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o_tmem + c * 16, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st16(o_tmem + c * 16, o);
+          }
+        }
+        const float neg = m == -INFINITY ? 0.f : -m;
+        const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2), ng2 = f2_pack(neg, neg);
+        uint64_t sum2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const int at = c * 32 + 2 * k;
+            const uint64_t x2 =
+                f2_fma(f2_pack(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])), sc2, ng2);
+            float e0, e1;
+            if ((k & 3) == 3) {
+              exp2_pair(x2, e0, e1);
+            } else {
+              f2_unpack(x2, e0, e1);
+              e0 = fast_exp2(e0);
+              e1 = fast_exp2(e1);
+            }
+            sum2[k & 1] = f2_add(sum2[k & 1], f2_pack(e0, e1));
+            pk[k] = pack2<T>(e0, e1);
+          }
+          tmem_st16(s_tmem + c * 16, pk);
+          if (c == 2) {  // P.V may start on three quarters of the keys
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&p_ready[x]);
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_rest[x]);
         float a0, a1, b0, b1;
         f2_unpack(sum2[0], a0, a1);
         f2_unpack(sum2[1], b0, b1);
         l += (a0 + b0) + (a1 + b1);
       }
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(&p_ready[x]);
-    }
-    ml_s[x * 128 + r] = make_float2(m, l);
-    mbar_arrive(&ml_full[x]);
-  } else {
-    // -------------------------------------------------------- correction --
-    setmaxnreg_dec<C::kRegsCorrection>();
-    const int r = static_cast<int>(threadIdx.x) - 256;
-    const uint32_t lane_base = tmem + 256 + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    bool ok = true;
-    for (int j = 0; j < nt && ok; ++j) {
-      for (int x = 0; x < (two ? 2 : 1); ++x) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&alpha_full[x], j & 1, p.err, abort_flag, kErrTimeoutSoftmax));
-        if (!ok) break;
-        const float a = alpha_s[x * 128 + r];
-        // (S(j) follows P.V(j - 1) in the tensor pipe: this one is over by now)
-        if (j > 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&o_done[x], (j - 1) & 1, p.err, abort_flag, kErrTimeoutSoftmax));
-          if (!ok) break;
-        }
-        if (j > 0 && __any_sync(0xffffffffu, a != 1.f)) {
-          tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(lane_base + x * 128 + c * 32, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * a);
-            tmem_st32(lane_base + x * 128 + c * 32, o);
-          }
-          tmem_st_wait();
-          tc_fence_before();
-        }
-        mbar_arrive(&p_ready[x]);
-      }
-    }
-    // ---------------------------------------------------------- epilogue --
-    for (int x = 0; x < (two ? 2 : 1) && ok; ++x) {
-      ok = __all_sync(0xffffffffu, mbar_wait(&ml_full[x], 0, p.err, abort_flag, kErrTimeoutSoftmax)) &&
-           __all_sync(0xffffffffu, mbar_wait(&o_done[x], (nt - 1) & 1, p.err, abort_flag, kErrTimeoutEpilogue));
       if (!ok) break;
+      // ------------------------------------------------------------ output --
+      ok = wait(&o_full[x], outputs & 1);
+      if (!ok) break;
+      ++outputs;
       tc_fence_after();
-      const float2 ml = ml_s[x * 128 + r];
       const int row = x * tok * p.G + r;
-      const bool valid = r < tok * p.G && row < rows;
-      if (pieces == 1) {
-        const float inv = inverse_sum(ml.y);
-        const int tr = (valid ? row : 0) / p.G, h = hk * p.G + (valid ? row : 0) % p.G;
-        const long long t = s.t0 + first + tr;
-        T* dst = static_cast<T*>(p.out) + t * p.os_t + h * p.os_h;
+      const bool valid = r < tok * p.G && row < w.count * p.G;
+      const int tr = row / p.G, h = w.hk * p.G + row - tr * p.G;
+      const long long t = w.s.t0 + w.first + tr;
+      const bool whole = w.pieces == 1;
+      const long long part = static_cast<long long>(w.slot) * 256 + row;
+      if (!*reinterpret_cast<volatile int*>(&work[item & 1].by_hand)) {
+        // Through shared memory, 128 bytes of each of the warp's 32 rows at a
+        // time (16-byte chunks swizzled by row), so that rows leave as whole
+        // 128-byte lines: lane 8 q + c has chunk c of rows q, q + 4, ...
+        const float inv = whole ? inverse_sum(l) : 1.f;
+        uint8_t* mine = !valid ? nullptr
+                        : whole ? reinterpret_cast<uint8_t*>(static_cast<T*>(p.out) + t * p.os_t + h * p.os_h)
+                                : reinterpret_cast<uint8_t*>(p.part_o + part * DP);
+        uint8_t* to[8];
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
+        for (int q = 0; q < 8; ++q)
+          to[q] = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine),
+                                                         q * 4 + (lane >> 3)));
+        const int row_bytes = whole ? p.D * 2 : DP * 4;
+#pragma unroll 1
+        for (int c0 = 0; c0 < (whole ? DP / 64 : DP / 32); ++c0) {
           uint32_t o[32];
-          tmem_ld32(lane_base + x * 128 + c * 32, o);
-          tmem_ld_wait();
-          if (valid) {
+          if (whole) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-              if (c * 32 + k < p.D) {
-                uint4 w;
-                w.x = pack2<T>(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
-                w.y = pack2<T>(__uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
-                w.z = pack2<T>(__uint_as_float(o[k + 4]) * inv, __uint_as_float(o[k + 5]) * inv);
-                w.w = pack2<T>(__uint_as_float(o[k + 6]) * inv, __uint_as_float(o[k + 7]) * inv);
-                *reinterpret_cast<uint4*>(dst + c * 32 + k) = w;
+            for (int half = 0; half < 2; ++half) {
+              tmem_ld32(o_tmem + c0 * 64 + half * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                uint4 v;
+                v.x = pack2<T>(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv);
+                v.y = pack2<T>(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
+                v.z = pack2<T>(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
+                v.w = pack2<T>(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
+                *reinterpret_cast<uint4*>(stage + lane * 128 + (((half * 4 + k) ^ (lane & 7)) << 4)) = v;
               }
             }
+          } else {
+            tmem_ld32(o_tmem + c0 * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4)) =
+                  make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
+          __syncwarp();
+          uint4 v[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const int rr = q * 4 + (lane >> 3);
+            v[q] = *reinterpret_cast<const uint4*>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+          }
+          const int at = c0 * 128 + (lane & 7) * 16;
+          const bool in_row = at < row_bytes;
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (to[q] && in_row) *reinterpret_cast<uint4*>(to[q] + at) = v[q];
+          __syncwarp();
         }
-        if (valid && p.lse) p.lse[t * p.Hq + h] = log_sum(ml.x, ml.y);
+        if (valid) {
+          if (!whole) p.part_ml[part] = make_float2(m, l);
+          else if (p.lse) p.lse[t * p.Hq + h] = log_sum(m, l);
+        }
       } else {
-        const long long at = (static_cast<long long>(entry) * p.splits + split) * 256 + row;
+        const int row0 = x * tok * p.G + (warp & 3) * 32;
+        for (int rr = row0; rr < min(row0 + 32, min((x + 1) * tok, w.count) * p.G); ++rr) {
+          const int tk = w.first + rr / p.G, hh = w.hk * p.G + rr % p.G;
+          const long long tt = w.s.t0 + tk;
+          float me, le, o[DP / 32];
+          exact_row<T, DP>(p, w.b, w.hk, static_cast<const T*>(p.q) + tt * p.qs_t + hh * p.qs_h,
+                           max(w.tile0 * KT, key_lo(p, w.s, tk)),
+                           min((w.tile0 + w.nt) * KT, key_hi(p, w.s, tk)), me, le, o);
+          const long long at = static_cast<long long>(w.slot) * 256 + rr;
+          const float inv = inverse_sum(le);
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(lane_base + x * 128 + c * 32, o);
-          tmem_ld_wait();
-          if (valid) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<uint4*>(p.part_o + at * DP + c * 32 + k) =
-                  make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          for (int c = 0; c < DP / 32; ++c) {
+            const int d = lane + c * 32;
+            if (!whole) p.part_o[at * DP + d] = o[c];
+            else if (d < p.D)
+              reinterpret_cast<uint16_t*>(static_cast<T*>(p.out) + tt * p.os_t + hh * p.os_h)[d] =
+                  static_cast<uint16_t>(pack2<T>(o[c] * inv, 0.f));
+          }
+          if (lane == 0) {
+            if (!whole) p.part_ml[at] = make_float2(me, le);
+            else if (p.lse) p.lse[tt * p.Hq + hh] = log_sum(me, le);
           }
         }
-        if (valid) p.part_ml[at] = ml;
       }
+      tc_fence_before();
+      release_work();
     }
-    tc_fence_before();
+  } else {
+    // ---------------------------------------------- values of masked tiles --
+    // 0 * inf and 0 * NaN are NaN: value rows past the sequence's end (stale
+    // memory) are cleared; where another masked value is not finite, the item's
+    // rows are formed one by one instead.
+    setmaxnreg_dec<C::kRegsValues>();
+    const int t = static_cast<int>(threadIdx.x) - 256;
+    uint32_t place = 0, looked = 0;  // looked: phases of v_look, a bit per stage
+    while (ok && next_work()) {
+      const TileWork w = work[item & 1];
+      for (int j = 0; j < w.nt && ok; ++j, place += 2) {
+        if (!masked(w, j)) continue;
+        const uint32_t at = place + 1, st = at % STAGES;
+        ok = wait(&v_look[st], (looked >> st) & 1) &&
+             wait(&full[st], (at / STAGES) & 1);
+        if (!ok) break;
+        looked ^= 1u << st;
+        uint8_t* v = smem + C::OFF_KV + st * C::TILE;
+        const int live = w.s.len - (w.tile0 + j) * KT;  // key rows of the sequence
+        uint32_t bad = 0;
+#pragma unroll
+        for (int c = 0; c < C::HALVES; ++c) {
+          uint4 u[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) u[k] = *reinterpret_cast<const uint4*>(v + c * (KT * 128) + (k * 128 + t) * 16);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int key = k * 16 + (t >> 3);
+            if (key < live) bad |= not_finite4<T>(u[k]);
+            else *reinterpret_cast<uint4*>(v + c * (KT * 128) + (k * 128 + t) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+        }
+        if (bad) *reinterpret_cast<volatile int*>(&work[item & 1].by_hand) = 1;
+        fence_proxy_async_smem();
+        mbar_arrive(&v_fixed[st]);
+      }
+      if (ok) release_work();
+    }
   }
 
+  if (late && lane == 0)
+    atomicCAS(p.err, 0, warp < 8 ? kErrTimeoutSoftmax : warp < 12 ? kErrTimeoutConvert
+                        : warp == 13 ? kErrTimeoutMma : kErrTimeoutProducer);
+  // Back to 128 registers a thread; those that grow wait until the softmax
+  // warps have given theirs up.
   tc_fence_before();
-  // Back to 128 registers a thread for the common tail; those that grow wait
-  // until the softmax warps have given theirs up.
   if (warp < 8) setmaxnreg_dec<128>();
   __syncthreads();
   if (warp >= 8) setmaxnreg_inc<128>();
   if (warp == 13) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
-  }
-  if (*by_hand && !*abort_flag) {
-    for (int row = warp; row < rows; row += C::kThreads / 32) {
-      const int tr = first + row / p.G, h = hk * p.G + row % p.G;
-      const long long t = s.t0 + tr;
-      const T* q = static_cast<const T*>(p.q) + t * p.qs_t + h * p.qs_h;
-      float m, l, o[DP / 32];
-      exact_row<T, DP>(p, b, hk, q, max(tile0 * KT, key_lo(p, s, tr)), min(tile1 * KT, key_hi(p, s, tr)), m, l, o);
-      const long long at = (static_cast<long long>(entry) * p.splits + split) * 256 + row;
-      const float inv = inverse_sum(l);
-#pragma unroll
-      for (int c = 0; c < DP / 32; ++c) {
-        const int d = lane + c * 32;
-        if (pieces > 1) p.part_o[at * DP + d] = o[c];
-        else if (d < p.D)
-          reinterpret_cast<uint16_t*>(static_cast<T*>(p.out) + t * p.os_t + h * p.os_h)[d] =
-              static_cast<uint16_t>(pack2<T>(o[c] * inv, 0.f));
-      }
-      if (lane == 0) {
-        if (pieces > 1) p.part_ml[at] = make_float2(m, l);
-        else if (p.lse) p.lse[t * p.Hq + h] = log_sum(m, l);
-      }
-    }
   }
 }
 
