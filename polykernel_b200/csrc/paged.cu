@@ -42,12 +42,15 @@ rotary::RowShape row_shape(int D, int half, int interleaved, int p) {
   return r;
 }
 
-// Heads that one thread visits: as many (up to 8) as still leave every SM
-// about a thousand threads. The sines of a pair are computed once per thread.
-int heads_per_thread(long long threads_per_head, int heads, int sms) {
-  int n = 1;
-  while (n < 8 && threads_per_head * ((heads + 2 * n - 1) / (2 * n)) >= 1024LL * sms) n *= 2;
-  return n;
+// How many of a token's `heads` rows a thread takes: four, for which it forms the
+// cosines once, unless that leaves the SMs without threads.
+rotary::Share share_of(const rotary::RowShape& r, long long tokens, int heads, int sms, bool token_first) {
+  rotary::Share s;
+  s.rows = rotary::kRows;
+  while (s.rows > 1 && tokens * r.items * ((heads + s.rows - 1) / s.rows) < 1024LL * sms) s.rows /= 2;
+  s.lanes = (heads + s.rows - 1) / s.rows;
+  s.token_first = token_first;
+  return s;
 }
 
 template <typename T>
@@ -327,11 +330,10 @@ int pkb200_rope(const void* x, void* y, int dtype, const long long* positions,
   a.row = row_shape(D, rot_pairs, interleaved, p);
   a.factor = factor;
   a.backward = backward;
-  a.heads_per_thread = heads_per_thread(tokens * a.row.items * B, H, sms);
-  const long long blocks = (tokens * a.row.items + 255) / 256;
-  const int groups = (H + a.heads_per_thread - 1) / a.heads_per_thread;
-  if (blocks > 0x7fffffffLL || groups > 65535) return cudaErrorInvalidValue;
-  const dim3 grid(static_cast<unsigned>(blocks), groups, B);
+  a.share = share_of(a.row, tokens * B, H, sms, a.xs_s < a.xs_h);
+  const long long blocks = (tokens * a.share.lanes * a.row.items + 255) / 256;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(blocks), B);
   if (dtype == PKB200_BF16) launch_rope<__nv_bfloat16>(p, grid, S(stream), a);
   else if (dtype == PKB200_FP16) launch_rope<__half>(p, grid, S(stream), a);
   else launch_rope<float>(p, grid, S(stream), a);
@@ -400,14 +402,10 @@ int pkb200_paged_kv_append(const pkb200_paged_cache* cache, const pkb200_paged_b
   a.row = row_shape(cache->dim, rot_pairs, interleaved, p);
   a.factor = factor;
   a.err = err;
-  const long long per_head = static_cast<long long>(a.T) * a.row.items;
-  a.heads_per_thread = heads_per_thread(per_head, q_heads + 2 * cache->heads, sms);
-  a.q_groups = (q_heads + a.heads_per_thread - 1) / a.heads_per_thread;
-  a.kv_groups = (cache->heads + a.heads_per_thread - 1) / a.heads_per_thread;
-  const long long blocks = (per_head + 255) / 256;
-  const long long groups = a.q_groups + 2LL * a.kv_groups;
-  if (blocks > 0x7fffffffLL || groups > 65535) return cudaErrorInvalidValue;
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(groups));
+  a.share = share_of(a.row, a.T, q_heads + 2 * cache->heads, sms, false);
+  const long long blocks = (static_cast<long long>(a.T) * a.share.lanes * a.row.items + 255) / 256;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(blocks));
   if (cache->dtype == PKB200_BF16) launch_append<__nv_bfloat16>(p, grid, S(stream), a);
   else launch_append<__half>(p, grid, S(stream), a);
   internal::count_launch(internal::kOther);

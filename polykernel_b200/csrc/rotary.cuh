@@ -9,9 +9,10 @@
 // copied. Arithmetic in fp32, one rounding at the end.
 //
 // Both kernels are bound by HBM (one read and one write per value). The angles
-// are therefore computed here, from 4 bytes of frequency per pair, instead of
-// being read from a table; one thread keeps the cosines of its pairs for all
-// the heads that it visits.
+// are computed here, from 4 bytes of frequency per pair, instead of being read
+// from a table; a thread keeps the cosines of its pairs for the head rows (up
+// to four) that it moves. No thread waits for another, and registers are kept
+// to four blocks per SM: the loads in flight are what the bandwidth needs.
 #pragma once
 
 #include "paged_index.h"
@@ -68,17 +69,17 @@ __device__ __forceinline__ void item_offsets(const RowShape& s, int item, int& u
   }
 }
 
-// cos and sin of one item's pairs at `position`. The angle in turns is formed
-// in 64 bits and reduced there: position * frequency has no fraction left in
-// 32 bits once it passes 2^24 radians, and only 8 bits of one at 2^16.
+// cos and sin of one item's pairs at `position`. The angle in turns is formed in
+// 64 bits and reduced there: position * frequency has no fraction left in 32
+// bits once it passes 2^24 radians, and only 8 bits of one at 2^16.
 template <int P>
-__device__ __forceinline__ void angles(const float* __restrict__ inv_freq, int item, long long position,
-                                       float factor, bool backward, float (&c)[P], float (&s)[P]) {
+__device__ __forceinline__ void angles(const float* __restrict__ inv_freq, long long position, float factor,
+                                       bool backward, float (&c)[P], float (&s)[P]) {
   constexpr double kTurnsPerRadian = 0.15915494309189533577;  // 1 / (2 pi)
-  const double pos = static_cast<double>(position);
+  const double pos = static_cast<double>(position) * kTurnsPerRadian;
 #pragma unroll
   for (int k = 0; k < P; ++k) {
-    const double turns = pos * (static_cast<double>(__ldg(inv_freq + item * P + k)) * kTurnsPerRadian);
+    const double turns = pos * static_cast<double>(__ldg(inv_freq + k));
     const float part = static_cast<float>(turns - rint(turns));  // in [-1/2, 1/2]
     float sn, cs;
     sincospif(2.f * part, &sn, &cs);
@@ -112,33 +113,74 @@ __device__ __forceinline__ void turn(Unit<T, P>& x, Unit<T, P>& y, const float (
   }
 }
 
-// Head rows that one thread has in flight: it issues their loads together.
-constexpr int kFlight = 4;
+// A thread moves one item of the rows lane, lane + lanes, ... of a token's (at
+// most `rows` of them). Threads are numbered by item first, then by token and
+// lane in the order of the strides.
+struct Share {
+  int lanes, rows;
+  int token_first;  // neighbours take the next token, not the next lane
+};
+constexpr int kFlight = 2;  // rows whose loads a thread has under way at once
+constexpr int kRows = 4;    // most rows of a thread
 
-// Moves one item of `heads` rows from src to dst (rotated when asked).
-template <typename T, int P>
-__device__ __forceinline__ void move_rows(const T* src, long long src_stride, T* dst,
-                                          long long dst_stride, int heads, int u0, int u1, bool two,
-                                          bool rotate, bool interleaved, const float (&c)[P],
-                                          const float (&s)[P]) {
+struct Place {
+  long long token;
+  int lane, item;
+};
+__device__ __forceinline__ Place place_of(long long index, const RowShape& r, const Share& s, long long tokens) {
+  Place p;
+  long long rest;
+  if (index <= 0x7fffffff) {  // 32-bit division where it will do
+    const unsigned i = static_cast<unsigned>(index), items = r.items;
+    rest = i / items;
+    p.item = static_cast<int>(i - static_cast<unsigned>(rest) * items);
+    const unsigned q = static_cast<unsigned>(rest), d = s.token_first ? static_cast<unsigned>(tokens) : s.lanes;
+    const unsigned hi = q / d, lo = q - hi * d;
+    p.token = s.token_first ? lo : hi;
+    p.lane = s.token_first ? hi : lo;
+    return p;
+  }
+  rest = index / r.items;
+  p.item = static_cast<int>(index - rest * r.items);
+  const long long d = s.token_first ? tokens : s.lanes, hi = rest / d, lo = rest - hi * d;
+  p.token = s.token_first ? lo : hi;
+  p.lane = static_cast<int>(s.token_first ? hi : lo);
+  return p;
+}
+
+// Moves one item of a thread's rows. `source(i)` gives the i-th row, or null;
+// `ready` looks up what `target(i)` (null: drop the row) and the cosines need,
+// while the first rows are on their way.
+template <typename T, int P, class Source, class Ready, class Target, class Turns>
+__device__ __forceinline__ void move_rows(const RowShape& s, int item, int rows, Source source, Ready ready,
+                                          Target target, Turns turns) {
   using U = Unit<T, P>;
-  for (int h0 = 0; h0 < heads; h0 += kFlight) {
-    U x[kFlight], y[kFlight];
+  int u0, u1;
+  bool two;
+  item_offsets<P>(s, item, u0, u1, two);
+  U x[kFlight], y[kFlight];
+  auto load = [&](int i0) {
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
-      if (h0 + i < heads) {
-        const T* row = src + (h0 + i) * src_stride;
-        x[i] = *reinterpret_cast<const U*>(row + u0);
-        if (two) y[i] = *reinterpret_cast<const U*>(row + u1);
+      const T* src = i0 + i < rows ? source(i0 + i) : nullptr;
+      if (src) {
+        x[i] = *reinterpret_cast<const U*>(src + u0);
+        if (two) y[i] = *reinterpret_cast<const U*>(src + u1);
       }
     }
+  };
+  load(0);
+  float c[P], sn[P];
+  if (!ready(c, sn)) return;
+  for (int i0 = 0; i0 < rows; i0 += kFlight) {
+    if (i0) load(i0);
 #pragma unroll
     for (int i = 0; i < kFlight; ++i) {
-      if (h0 + i < heads) {
-        if (rotate) turn<T, P>(x[i], y[i], c, s, interleaved);
-        T* row = dst + (h0 + i) * dst_stride;
-        *reinterpret_cast<U*>(row + u0) = x[i];
-        if (two) *reinterpret_cast<U*>(row + u1) = y[i];
+      T* dst = i0 + i < rows ? target(i0 + i) : nullptr;
+      if (dst) {
+        if (turns(i0 + i)) turn<T, P>(x[i], y[i], c, sn, s.interleaved != 0);
+        *reinterpret_cast<U*>(dst + u0) = x[i];
+        if (two) *reinterpret_cast<U*>(dst + u1) = y[i];
       }
     }
   }
@@ -152,33 +194,33 @@ struct RopeParams {
   const float* inv_freq;
   long long xs_b, xs_s, xs_h, ys_b, ys_s, ys_h;  // strides, in values
   long long S;
-  int H, heads_per_thread;
+  int H;
   RowShape row;
+  Share share;
   float factor;
   int backward;
 };
 
-// grid: x over (token, item), y over groups of heads, z over the batch.
+// grid: x over the shares of one batch entry, y over the batch.
 template <typename T, int P>
-__global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
-  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const long long token = i / p.row.items;
-  if (token >= p.S) return;
-  const int item = static_cast<int>(i - token * p.row.items);
-  const int h0 = blockIdx.y * p.heads_per_thread;
-  const int heads = min(p.heads_per_thread, p.H - h0);
-  int u0, u1;
-  bool two;
-  item_offsets<P>(p.row, item, u0, u1, two);
-  const bool rotate = item < p.row.rot_items;
-  float c[P], s[P];
-  if (rotate)
-    angles<P>(p.inv_freq, item, p.positions[blockIdx.z * p.pos_stride_b + token], p.factor,
-              p.backward != 0, c, s);
-  const long long b = blockIdx.z;
-  move_rows<T, P>(static_cast<const T*>(p.x) + b * p.xs_b + token * p.xs_s + h0 * p.xs_h, p.xs_h,
-                  static_cast<T*>(p.y) + b * p.ys_b + token * p.ys_s + h0 * p.ys_h, p.ys_h, heads, u0,
-                  u1, two, rotate, p.row.interleaved != 0, c, s);
+__global__ void __launch_bounds__(256, 4) rope_kernel(const RopeParams p) {
+  const long long index = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (index >= p.S * p.share.lanes * p.row.items) return;
+  const Place at = place_of(index, p.row, p.share, p.S);
+  const long long b = blockIdx.y;
+  const T* src = static_cast<const T*>(p.x) + b * p.xs_b + at.token * p.xs_s + at.lane * p.xs_h;
+  T* dst = static_cast<T*>(p.y) + b * p.ys_b + at.token * p.ys_s + at.lane * p.ys_h;
+  const bool rotated = at.item < p.row.rot_items;
+  const int rows = min(p.share.rows, (p.H - at.lane + p.share.lanes - 1) / p.share.lanes);
+  move_rows<T, P>(
+      p.row, at.item, rows, [&](int i) { return src + i * p.share.lanes * p.xs_h; },
+      [&](float(&c)[P], float(&s)[P]) {
+        if (rotated)
+          angles<P>(p.inv_freq + at.item * P, p.positions[b * p.pos_stride_b + at.token], p.factor,
+                    p.backward != 0, c, s);
+        return true;
+      },
+      [&](int i) { return dst + i * p.share.lanes * p.ys_h; }, [&](int) { return rotated; });
 }
 
 struct AppendParams {
@@ -192,73 +234,63 @@ struct AppendParams {
   const int* lens;
   const float* inv_freq;
   int T, B, Hq, Hkv, page_size, num_pages, table_width;
-  int heads_per_thread, q_groups, kv_groups;  // y: q groups, then k groups, then v groups
   RowShape row;
+  Share share;
   float factor;
   int* err;
 };
 
-// Sequences whose offsets one block keeps in shared memory for its lookups;
-// a larger batch is searched in global memory.
-constexpr int kAppendSeqs = 2048;
-
-// grid: x over (token, item), y over groups of q, k and v heads.
+// grid: x over the shares; the q, k and v heads of a token are numbered through.
 template <typename T, int P>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
-  __shared__ int cu_s[kAppendSeqs + 1];
-  const bool shared = p.B <= kAppendSeqs;
-  if (shared) {
-    for (int i = threadIdx.x; i <= p.B; i += blockDim.x) cu_s[i] = __ldg(p.cu + i);
-    __syncthreads();
-  }
-  const int* cu = shared ? cu_s : p.cu;
-  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const long long token = i / p.row.items;
-  if (token >= p.T) return;
-  const int item = static_cast<int>(i - token * p.row.items);
-  int seq;
-  long long position;
-  const auto place = paged::place_token(cu, p.B, token, [&](int b) { return __ldg(p.lens + b); }, seq, position);
-  if (place != paged::kPlaced) {  // rows of no sequence stay as they are
-    if (place == paged::kMisplaced && item == 0) atomicCAS(p.err, 0, kErrBadBatch);
-    return;
-  }
-  int u0, u1;
-  bool two;
-  item_offsets<P>(p.row, item, u0, u1, two);
-  const int group = blockIdx.y;
-  const bool is_q = group < p.q_groups;
-  const bool is_v = group >= p.q_groups + p.kv_groups;
-  const bool rotate = !is_v && item < p.row.rot_items;
-  float c[P], s[P];
-  if (rotate) angles<P>(p.inv_freq, item, position, p.factor, false, c, s);
-  const bool il = p.row.interleaved != 0;
-  if (is_q) {
-    const int h0 = group * p.heads_per_thread;
-    move_rows<T, P>(static_cast<const T*>(p.q) + token * p.qs_t + h0 * p.qs_h, p.qs_h,
-                    static_cast<T*>(p.q_out) + token * p.os_t + h0 * p.os_h, p.os_h,
-                    min(p.heads_per_thread, p.Hq - h0), u0, u1, two, rotate, il, c, s);
-    return;
-  }
-  const long long slot = position / p.page_size;
-  const int page =
-      slot < p.table_width ? paged::clip_page(__ldg(p.page_table + seq * p.table_stride + slot), p.num_pages)
-                           : p.num_pages;
-  if (page == p.num_pages) {
-    if (item == 0) atomicCAS(p.err, 0, kErrBadBatch);
-    return;
-  }
-  const int row = static_cast<int>(position - slot * p.page_size);
-  const int h0 = (group - p.q_groups - (is_v ? p.kv_groups : 0)) * p.heads_per_thread;
-  const int heads = min(p.heads_per_thread, p.Hkv - h0);
-  if (is_v)
-    move_rows<T, P>(static_cast<const T*>(p.v) + token * p.vs_t + h0 * p.vs_h, p.vs_h,
-                    static_cast<T*>(p.v_pages) + page * p.vp_p + row * p.vp_r + h0 * p.vp_h, p.vp_h,
-                    heads, u0, u1, two, false, il, c, s);
-  else
-    move_rows<T, P>(static_cast<const T*>(p.k) + token * p.ks_t + h0 * p.ks_h, p.ks_h,
-                    static_cast<T*>(p.k_pages) + page * p.kp_p + row * p.kp_r + h0 * p.kp_h, p.kp_h,
-                    heads, u0, u1, two, rotate, il, c, s);
+__global__ void __launch_bounds__(256, 4) paged_append_kernel(const AppendParams p) {
+  const long long index = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (index >= static_cast<long long>(p.T) * p.share.lanes * p.row.items) return;
+  const Place at = place_of(index, p.row, p.share, p.T);
+  const long long token = at.token;
+  const int all = p.Hq + 2 * p.Hkv;
+  const int rows = min(p.share.rows, (all - at.lane + p.share.lanes - 1) / p.share.lanes);
+  const bool rotated = at.item < p.row.rot_items;
+  auto head = [&](int i) { return at.lane + i * p.share.lanes; };
+  T *k_row = nullptr, *v_row = nullptr;  // this token's row of head 0 in the pools, null to drop it
+  move_rows<T, P>(
+      p.row, at.item, rows,
+      [&](int i) {
+        const int h = head(i);
+        return h < p.Hq           ? static_cast<const T*>(p.q) + token * p.qs_t + h * p.qs_h
+               : h < p.Hq + p.Hkv ? static_cast<const T*>(p.k) + token * p.ks_t + (h - p.Hq) * p.ks_h
+                                  : static_cast<const T*>(p.v) + token * p.vs_t + (h - p.Hq - p.Hkv) * p.vs_h;
+      },
+      [&](float(&c)[P], float(&s)[P]) {
+        int seq;
+        long long position;
+        const auto where =
+            paged::place_token(p.cu, p.B, token, [&](int b) { return __ldg(p.lens + b); }, seq, position);
+        if (where != paged::kPlaced) {  // rows of no sequence stay as they are
+          if (where == paged::kMisplaced) atomicCAS(p.err, 0, kErrBadBatch);
+          return false;
+        }
+        long long slot = position / p.page_size;
+        const int row = static_cast<int>(position - slot * p.page_size);
+        const int page = slot < p.table_width
+                             ? paged::clip_page(__ldg(p.page_table + seq * p.table_stride + slot), p.num_pages)
+                             : p.num_pages;
+        if (page < p.num_pages) {
+          k_row = static_cast<T*>(p.k_pages) + page * p.kp_p + row * p.kp_r;
+          v_row = static_cast<T*>(p.v_pages) + page * p.vp_p + row * p.vp_r;
+        } else {
+          atomicCAS(p.err, 0, kErrBadBatch);
+        }
+        if (rotated) angles<P>(p.inv_freq + at.item * P, position, p.factor, false, c, s);
+        return true;
+      },
+      [&](int i) -> T* {
+        const int h = head(i);
+        return h < p.Hq    ? static_cast<T*>(p.q_out) + token * p.os_t + h * p.os_h
+               : !k_row    ? nullptr
+               : h < p.Hq + p.Hkv ? k_row + (h - p.Hq) * p.kp_h
+                                  : v_row + (h - p.Hq - p.Hkv) * p.vp_h;
+      },
+      [&](int i) { return rotated && head(i) < p.Hq + p.Hkv; });
 }
 
 }  // namespace rotary

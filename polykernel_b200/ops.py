@@ -398,5 +398,5 @@ def qkv_projection(x, w_qkv, num_heads):
 
 
 # Ragged batches over a paged cache (polykernel_b200/paged.py).
-from .paged import (paged_attention, paged_kv_append, rope, rope_backward,  # noqa: E402,F401
-                    rope_frequencies)
+from .paged import (load_paged, paged_attention, paged_kv_append, rope,  # noqa: E402,F401
+                    rope_backward, rope_frequencies)

@@ -17,51 +17,34 @@ fused projection, with a contiguous last axis.
 """
 from __future__ import annotations
 
-import ctypes
+import glob
+import importlib.machinery
+import importlib.util
 import math
+import os
 
 import torch
 
-from ._lib import PagedBatch, PagedCache, check, lib
+from ._lib import LIB_PATH, lib
 
-_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-_LL2, _LL3 = ctypes.c_longlong * 2, ctypes.c_longlong * 3
-
-
-def _tensor(t, name, dtypes, dims, device=None):
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if t.dtype not in dtypes:
-        raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if t.dim() != dims:
-        raise ValueError(f"{name} must have {dims} dims, got shape {tuple(t.shape)}")
-    return t
+_module = None
 
 
-def _rows(t, name, dtype, device, shape):
-    """A tensor [tokens, heads, dim] with a contiguous last axis."""
-    _tensor(t, name, (dtype,), len(shape), device)
-    if t.shape != shape:
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    return _last(t, name)
-
-
-def _last(t, name):
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{name} must have a contiguous last axis")
-    return t
-
-
-def _call(device, f, *args):
-    """f(*args, stream) on the tensors' device and its current stream."""
-    if device.index == torch.cuda.current_device():
-        return f(*args, torch.cuda.current_stream().cuda_stream)
-    with torch.cuda.device(device):
-        return f(*args, torch.cuda.current_stream().cuda_stream)
+def load_paged():
+    """The compiled module (csrc/paged_binding.cpp), loaded once; raises if it is not built."""
+    global _module
+    if _module is None:
+        lib()  # the library that it calls
+        found = glob.glob(os.path.join(os.path.dirname(LIB_PATH), "_paged.*.so"))
+        if not found:
+            raise RuntimeError("pkb200: Python module of the paged operators not built; run "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`")
+        loader = importlib.machinery.ExtensionFileLoader("_paged", found[0])
+        spec = importlib.util.spec_from_file_location("_paged", found[0], loader=loader)
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+        _module = module
+    return _module
 
 
 def rope_frequencies(rot_dim, base=10000.0, scaling=None, device="cuda"):
@@ -124,47 +107,6 @@ def rope_frequencies(rot_dim, base=10000.0, scaling=None, device="cuda"):
     return f.float().to(device), float(factor)
 
 
-def _frequencies(inv_freq, device, dim):
-    _tensor(inv_freq, "inv_freq", (torch.float32,), 1, device)
-    if not inv_freq.is_contiguous():
-        raise ValueError("inv_freq must be contiguous")
-    if 2 * inv_freq.shape[0] > dim:
-        raise ValueError(f"inv_freq has {inv_freq.shape[0]} pairs for a head of {dim} values")
-    return inv_freq
-
-
-def _rope(x, positions, inv_freq, interleaved, factor, out, backward):
-    if not isinstance(x, torch.Tensor) or x.dim() not in (3, 4):
-        raise ValueError("x must be a tensor [T, H, D] or [B, H, S, D]")
-    _last(_tensor(x, "x", tuple(_DTYPES), x.dim()), "x")
-    dev = x.device
-    packed = x.dim() == 3
-    B, S, H, D = (1, *x.shape) if packed else (x.shape[0], x.shape[2], x.shape[1], x.shape[3])
-    _frequencies(inv_freq, dev, D)
-    if not isinstance(positions, torch.Tensor) or positions.dim() not in (1, 2):
-        raise ValueError("positions must be a tensor of one position per token")
-    _last(_tensor(positions, "positions", (torch.int64,), positions.dim(), dev), "positions")
-    if positions.shape[-1] != S or (positions.dim() == 2 and (packed or positions.shape[0] != B)):
-        raise ValueError(f"positions {tuple(positions.shape)} do not match x {tuple(x.shape)}")
-    if not math.isfinite(factor):
-        raise ValueError("factor must be finite")
-    if out is None:
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    else:
-        _rows(out, "out", x.dtype, dev, x.shape)
-        if out.data_ptr() == x.data_ptr() and out.stride() != x.stride():
-            raise ValueError("out may be x itself, not another view of its memory")
-
-    def strides(t):
-        return _LL3(0, t.stride(0), t.stride(1)) if packed else _LL3(t.stride(0), t.stride(2), t.stride(1))
-
-    check(_call(dev, lib().pkb200_rope, x.data_ptr(), out.data_ptr(), _DTYPES[x.dtype],
-                positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0,
-                inv_freq.data_ptr(), inv_freq.shape[0], B, S, H, D, strides(x), strides(out),
-                float(factor), int(bool(interleaved)), int(backward)), "rope")
-    return out
-
-
 def rope(x, positions, inv_freq, interleaved=False, factor=1.0, out=None):
     """Rotary positions. x is [T, H, D] (packed tokens) or [B, H, S, D] (what
     `qkv_projection` returns); positions int64 [T], [S] or [B, S]. The first
@@ -172,48 +114,13 @@ def rope(x, positions, inv_freq, interleaved=False, factor=1.0, out=None):
     (2i, 2i + 1) if interleaved, by position * inv_freq[i], and scaled by factor;
     the others are copied. Angles are exact for positions up to 2^31. `out` may
     be x."""
-    return _rope(x, positions, inv_freq, interleaved, factor, out, False)
+    return load_paged().rope(x, positions, inv_freq, interleaved, factor, out, False)
 
 
 def rope_backward(grad, positions, inv_freq, interleaved=False, factor=1.0, out=None):
     """The gradient of `rope` with respect to x, from that of its result: the
     rotation by the negative angles (arguments as for `rope`)."""
-    return _rope(grad, positions, inv_freq, interleaved, factor, out, True)
-
-
-def _paged(k_pages, v_pages, page_table, cu_seqlens, seq_lens, num_tokens):
-    """The C descriptions of the cache and the batch."""
-    _tensor(k_pages, "k_pages", (torch.bfloat16, torch.float16), 4)
-    dev = k_pages.device
-    _tensor(v_pages, "v_pages", (k_pages.dtype,), 4, dev)
-    if v_pages.shape != k_pages.shape:
-        raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} differ")
-    _last(k_pages, "k_pages")
-    _last(v_pages, "v_pages")
-    i32 = (torch.int32,)
-    _last(_tensor(page_table, "page_table", i32, 2, dev), "page_table")
-    _tensor(cu_seqlens, "cu_seqlens", i32, 1, dev)
-    _tensor(seq_lens, "seq_lens", i32, 1, dev)
-    B, width = page_table.shape
-    if cu_seqlens.shape[0] != B + 1 or seq_lens.shape[0] != B:
-        raise ValueError(f"page_table has {B} sequences, cu_seqlens {cu_seqlens.shape[0] - 1}, "
-                         f"seq_lens {seq_lens.shape[0]}")
-    if not (cu_seqlens.is_contiguous() and seq_lens.is_contiguous()):
-        raise ValueError("cu_seqlens and seq_lens must be contiguous")
-    pages, heads, page, dim = k_pages.shape
-    if heads == 0 or page == 0 or dim == 0:
-        raise ValueError(f"k_pages must have heads, rows and values, got {tuple(k_pages.shape)}")
-    cache = PagedCache(k_pages.data_ptr(), v_pages.data_ptr(), _LL3(*k_pages.stride()[:3]),
-                       _LL3(*v_pages.stride()[:3]), pages, heads, page, dim, _DTYPES[k_pages.dtype])
-    batch = PagedBatch(page_table.data_ptr(), cu_seqlens.data_ptr(), seq_lens.data_ptr(),
-                       page_table.stride(0), width, B, num_tokens)
-    return dev, cache, batch
-
-
-def _tokens(t, name):
-    if not isinstance(t, torch.Tensor) or t.dim() != 3:
-        raise ValueError(f"{name} must be a tensor [tokens, heads, dim]")
-    return t.shape[0]
+    return load_paged().rope(grad, positions, inv_freq, interleaved, factor, out, True)
 
 
 def paged_kv_append(k, v, k_pages, v_pages, page_table, cu_seqlens, seq_lens, inv_freq=None,
@@ -224,50 +131,8 @@ def paged_kv_append(k, v, k_pages, v_pages, page_table, cu_seqlens, seq_lens, in
     [T, q_heads, dim], whose rotation is returned (in `q_out`, which may be q; by
     default a new tensor, whose rows of no sequence are undefined).
     Two new tokens that share a cache row leave either's values there."""
-    n = _tokens(k, "k")
-    dev, cache, batch = _paged(k_pages, v_pages, page_table, cu_seqlens, seq_lens, n)
-    dt, heads, dim = k_pages.dtype, cache.heads, cache.dim
-    _rows(k, "k", dt, dev, (n, heads, dim))
-    _rows(v, "v", dt, dev, (n, heads, dim))
-    if inv_freq is None:
-        if q is not None or q_out is not None:
-            raise ValueError("q is only rotated: it needs inv_freq")
-        freq, pairs = None, 0
-    else:
-        freq, pairs = _frequencies(inv_freq, dev, dim).data_ptr(), inv_freq.shape[0]
-    if not math.isfinite(factor):
-        raise ValueError("factor must be finite")
-    q_args = (None, None, None, None, 0)
-    if q is not None:
-        hq = q.shape[1] if _tokens(q, "q") == n else -1
-        if hq <= 0:
-            raise ValueError(f"q must be [{n}, heads, {dim}], got {tuple(q.shape)}")
-        _rows(q, "q", dt, dev, (n, hq, dim))
-        if q_out is None:
-            q_out = torch.empty(n, hq, dim, dtype=dt, device=dev)
-        else:
-            _rows(q_out, "q_out", dt, dev, q.shape)
-            if q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride():
-                raise ValueError("q_out may be q itself, not another view of its memory")
-        q_args = (q.data_ptr(), _LL2(*q.stride()[:2]), q_out.data_ptr(), _LL2(*q_out.stride()[:2]), hq)
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    check(_call(dev, lib().pkb200_paged_kv_append, ctypes.byref(cache), ctypes.byref(batch),
-                k.data_ptr(), _LL2(*k.stride()[:2]), v.data_ptr(), _LL2(*v.stride()[:2]), *q_args,
-                freq, pairs, float(factor), int(bool(interleaved))), "paged_kv_append")
-    return q_out
-
-
-def _aligned(t, name):
-    """16-byte rows: what the copies of attention start on."""
-    if t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
-        raise ValueError(f"{name} must start on 16 bytes, with strides that are multiples of 8 values")
-    return t
-
-
-def _strides(t, make):
-    """Strides without the last axis's; those of axes of one are never taken."""
-    return make(*(s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape)))
+    return load_paged().paged_kv_append(k, v, k_pages, v_pages, page_table, cu_seqlens, seq_lens, inv_freq,
+                                  interleaved, factor, q, q_out)
 
 
 def paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, seq_lens, max_q_len=None, causal=True,
@@ -285,55 +150,5 @@ def paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, seq_lens, max_q
     speed (by default 1 for as many tokens as sequences, T otherwise).
     `workspace`: a uint8 tensor to use instead of a new one, if it is large enough;
     calls that may overlap need their own."""
-    n = _tokens(q, "q")
-    dev, cache, batch = _paged(k_pages, v_pages, page_table, cu_seqlens, seq_lens, n)
-    dim, hq = cache.dim, q.shape[1]
-    _rows(q, "q", k_pages.dtype, dev, (n, hq, dim))
-    if hq == 0 or hq % cache.heads:
-        raise ValueError(f"{hq} query heads do not divide among {cache.heads} key heads")
-    if dim % 8 or dim > 256:
-        raise ValueError(f"dim must be a multiple of 8 up to 256, got {dim}")
-    if cache.page_size % 8:
-        raise ValueError(f"the page size must be a multiple of 8, got {cache.page_size}")
-    if cache.num_pages == 0:
-        raise ValueError("k_pages has no pages")
-    if n * hq // cache.heads >= 2 ** 31 - 1:
-        raise ValueError("too many tokens for one call")
-    if window is not None and (window < 1 or not causal):
-        raise ValueError("window must be at least 1, and needs causal")
-    scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError("scale must be positive and finite")
-    if max_q_len is None:
-        max_q_len = 1 if n <= batch.num_seqs else n
-    elif max_q_len < 0:
-        raise ValueError("max_q_len must not be negative")
-    for t, name in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages")):
-        _aligned(t, name)
-    if out is None:
-        out = torch.empty(n, hq, dim, dtype=q.dtype, device=dev)
-    else:
-        _aligned(_rows(out, "out", q.dtype, dev, (n, hq, dim)), "out")
-    if lse is not None:
-        _tensor(lse, "lse", (torch.float32,), 2, dev)
-        if lse.shape != (n, hq) or not lse.is_contiguous():
-            raise ValueError(f"lse must be contiguous, of shape {(n, hq)}")
-    elif return_lse:
-        lse = torch.empty(n, hq, dtype=torch.float32, device=dev)
-    cache.k_stride, cache.v_stride = _strides(k_pages, _LL3), _strides(v_pages, _LL3)
-    window = min(window or 0, 2 ** 30)
-    max_q_len = min(max_q_len, n)
-
-    def go(stream):
-        nonlocal workspace
-        c, b = ctypes.byref(cache), ctypes.byref(batch)
-        need = lib().pkb200_paged_attention_workspace_size(c, b, hq, max_q_len, window)
-        if workspace is None or workspace.numel() < need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        return lib().pkb200_paged_attention(
-            c, b, q.data_ptr(), _strides(q, _LL2), out.data_ptr(), _strides(out, _LL2),
-            None if lse is None else lse.data_ptr(), hq, max_q_len, int(bool(causal)), window, scale,
-            workspace.data_ptr(), workspace.numel(), stream)
-
-    check(_call(dev, go), "paged_attention")
-    return (out, lse) if return_lse else out
+    return load_paged().paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, seq_lens, max_q_len, causal,
+                                  window, scale, return_lse, out, lse, workspace)
