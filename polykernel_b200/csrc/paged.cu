@@ -63,12 +63,12 @@ void launch_rope(int p, dim3 grid, cudaStream_t s, const rotary::RopeParams& a) 
   else rotary::rope_kernel<T, 1><<<grid, 256, 0, s>>>(a);
 }
 
-template <typename T>
+template <typename T, bool ROTATES>
 void launch_append(int p, dim3 grid, cudaStream_t s, const rotary::AppendParams& a) {
-  if (p == 8) rotary::paged_append_kernel<T, 8><<<grid, 256, 0, s>>>(a);
-  else if (p == 4) rotary::paged_append_kernel<T, 4><<<grid, 256, 0, s>>>(a);
-  else if (p == 2) rotary::paged_append_kernel<T, 2><<<grid, 256, 0, s>>>(a);
-  else rotary::paged_append_kernel<T, 1><<<grid, 256, 0, s>>>(a);
+  if (p == 8) rotary::paged_append_kernel<T, 8, ROTATES><<<grid, 256, 0, s>>>(a);
+  else if (p == 4) rotary::paged_append_kernel<T, 4, ROTATES><<<grid, 256, 0, s>>>(a);
+  else if (p == 2) rotary::paged_append_kernel<T, 2, ROTATES><<<grid, 256, 0, s>>>(a);
+  else rotary::paged_append_kernel<T, 1, ROTATES><<<grid, 256, 0, s>>>(a);
 }
 
 // What every paged entry point requires of the cache and the batch.
@@ -406,8 +406,10 @@ int pkb200_paged_kv_append(const pkb200_paged_cache* cache, const pkb200_paged_b
   const long long blocks = (static_cast<long long>(a.T) * a.share.lanes * a.row.items + 255) / 256;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(blocks));
-  if (cache->dtype == PKB200_BF16) launch_append<__nv_bfloat16>(p, grid, S(stream), a);
-  else launch_append<__half>(p, grid, S(stream), a);
+  // without a rotation the values are only moved: one 16-bit type does for both
+  if (rot_pairs == 0) launch_append<__half, false>(p, grid, S(stream), a);
+  else if (cache->dtype == PKB200_BF16) launch_append<__nv_bfloat16, true>(p, grid, S(stream), a);
+  else launch_append<__half, true>(p, grid, S(stream), a);
   internal::count_launch(internal::kOther);
   return cudaGetLastError();
 }

@@ -57,15 +57,23 @@ PKB_INDEX int clip_page(int page, int num_pages) {
   return page >= 0 && page < num_pages ? page : num_pages;
 }
 
-// Where the append puts a packed row: its sequence (the last that starts at or
-// before it), and its position there. kNoSequence: the row is of none;
+// Where the append puts a packed row: a sequence that has it, and its position there. kNoSequence: the row is of none;
 // kMisplaced: the offsets are out of order or the sequence is shorter than its
 // new tokens.
 enum TokenPlace { kPlaced, kNoSequence, kMisplaced };
 template <class Lengths>
 PKB_INDEX TokenPlace place_token(const int* cu, int num_seqs, long long token, Lengths lens, int& seq,
                                  long long& position) {
-  if (token < cu[0] || token >= cu[num_seqs]) return kNoSequence;
+  // With one new token each, which is what decoding steps have, it is sequence
+  // `token`: looked at first, with loads that do not wait for one another.
+  const int guess = token < num_seqs ? static_cast<int>(token) : num_seqs - 1;
+  const int begin = cu[0], end = cu[num_seqs], from = cu[guess], to = cu[guess + 1], len = lens(guess);
+  if (token < begin || token >= end) return kNoSequence;
+  if (token >= from && token < to) {
+    seq = guess;
+    position = static_cast<long long>(len) - to + token;
+    return position >= 0 ? kPlaced : kMisplaced;
+  }
   int lo = 0, hi = num_seqs;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;

@@ -21,22 +21,21 @@
 namespace pkb200 {
 namespace rotary {
 
+// Two 16-bit values in a word.
 template <typename T>
-__device__ __forceinline__ float to_f32(T v);
+__device__ __forceinline__ float2 unpack(uint32_t w);
 template <>
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
 template <>
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float2 unpack<__half>(uint32_t w) { return unpack_f16x2(w); }
 template <typename T>
-__device__ __forceinline__ T from_f32(float v);
+__device__ __forceinline__ uint32_t pack(float lo, float hi);
 template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float lo, float hi) { return pack_bf16x2(lo, hi); }
 template <>
-__device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ float from_f32(float v) { return v; }
+__device__ __forceinline__ uint32_t pack<__half>(float lo, float hi) { return pack_f16x2(lo, hi); }
 
 // A unit is P values that move as one access of P * sizeof(T) bytes.
 template <typename T, int P>
@@ -71,45 +70,84 @@ __device__ __forceinline__ void item_offsets(const RowShape& s, int item, int& u
 
 // cos and sin of one item's pairs at `position`. The angle in turns is formed in
 // 64 bits and reduced there: position * frequency has no fraction left in 32
-// bits once it passes 2^24 radians, and only 8 bits of one at 2^16.
-template <int P>
+// bits once it passes 2^24 radians, and only 8 bits of one at 2^16. For 16-bit
+// values the reduced angle goes to the SFU, whose error on [-pi, pi], 2^-21.4,
+// is far below their rounding (2^-9 and 2^-12); the accurate functions took
+// more instructions than everything else together.
+template <typename T, int P>
 __device__ __forceinline__ void angles(const float* __restrict__ inv_freq, long long position, float factor,
                                        bool backward, float (&c)[P], float (&s)[P]) {
   constexpr double kTurnsPerRadian = 0.15915494309189533577;  // 1 / (2 pi)
+  constexpr double kRound = 6755399441055744.0;               // 1.5 * 2^52: adding it rounds to whole numbers
+  constexpr float kTwoPi = 6.28318530717958648f;
   const double pos = static_cast<double>(position) * kTurnsPerRadian;
+  const float sign = backward ? -factor : factor;
 #pragma unroll
   for (int k = 0; k < P; ++k) {
     const double turns = pos * static_cast<double>(__ldg(inv_freq + k));
-    const float part = static_cast<float>(turns - rint(turns));  // in [-1/2, 1/2]
+    const float part = static_cast<float>(turns - ((turns + kRound) - kRound));  // in [-1/2, 1/2]
     float sn, cs;
-    sincospif(2.f * part, &sn, &cs);
+    if constexpr (sizeof(T) == 2) {
+      sn = __sinf(part * kTwoPi);
+      cs = __cosf(part * kTwoPi);
+    } else {
+      sincospif(2.f * part, &sn, &cs);
+    }
     c[k] = cs * factor;
-    s[k] = (backward ? -sn : sn) * factor;
+    s[k] = sn * sign;
   }
 }
 
+__device__ __forceinline__ void turn_pair(float& a, float& b, float c, float s) {
+  const float a0 = a;
+  a = a0 * c - b * s;
+  b = b * c + a0 * s;
+}
+
+// Rotates the P pairs that units x and y hold.
 template <typename T, int P>
-__device__ __forceinline__ void turn(Unit<T, P>& x, Unit<T, P>& y, const float (&c)[P],
-                                     const float (&s)[P], bool interleaved) {
-  if (interleaved) {
-    if constexpr (P >= 2) {
+__device__ __forceinline__ void turn(Unit<T, P>& x, Unit<T, P>& y, const float (&c)[P], const float (&s)[P],
+                                     bool interleaved) {
+  if constexpr (sizeof(T) == 4) {
+    if (interleaved && P >= 2) {
 #pragma unroll
       for (int k = 0; k < P / 2; ++k) {
-        const float a = to_f32(x.v[2 * k]), b = to_f32(x.v[2 * k + 1]);
-        x.v[2 * k] = from_f32<T>(a * c[k] - b * s[k]);
-        x.v[2 * k + 1] = from_f32<T>(b * c[k] + a * s[k]);
-        const float e = to_f32(y.v[2 * k]), f = to_f32(y.v[2 * k + 1]);
-        y.v[2 * k] = from_f32<T>(e * c[P / 2 + k] - f * s[P / 2 + k]);
-        y.v[2 * k + 1] = from_f32<T>(f * c[P / 2 + k] + e * s[P / 2 + k]);
+        turn_pair(x.v[2 * k], x.v[2 * k + 1], c[k], s[k]);
+        turn_pair(y.v[2 * k], y.v[2 * k + 1], c[P / 2 + k], s[P / 2 + k]);
       }
-      return;
-    }
-  }
+    } else {
 #pragma unroll
-  for (int k = 0; k < P; ++k) {
-    const float a = to_f32(x.v[k]), b = to_f32(y.v[k]);
-    x.v[k] = from_f32<T>(a * c[k] - b * s[k]);
-    y.v[k] = from_f32<T>(b * c[k] + a * s[k]);
+      for (int k = 0; k < P; ++k) turn_pair(x.v[k], y.v[k], c[k], s[k]);
+    }
+  } else if constexpr (P == 1) {  // one value each, whatever the layout
+    const uint32_t w = *reinterpret_cast<const uint16_t*>(&x) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&y)) << 16;
+    float2 v = unpack<T>(w);
+    turn_pair(v.x, v.y, c[0], s[0]);
+    const uint32_t r = pack<T>(v.x, v.y);
+    *reinterpret_cast<uint16_t*>(&x) = static_cast<uint16_t>(r);
+    *reinterpret_cast<uint16_t*>(&y) = static_cast<uint16_t>(r >> 16);
+  } else {
+    uint32_t* xw = reinterpret_cast<uint32_t*>(&x);
+    uint32_t* yw = reinterpret_cast<uint32_t*>(&y);
+    if (interleaved) {
+#pragma unroll
+      for (int k = 0; k < P / 2; ++k) {
+        float2 v = unpack<T>(xw[k]), w = unpack<T>(yw[k]);
+        turn_pair(v.x, v.y, c[k], s[k]);
+        turn_pair(w.x, w.y, c[P / 2 + k], s[P / 2 + k]);
+        xw[k] = pack<T>(v.x, v.y);
+        yw[k] = pack<T>(w.x, w.y);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < P / 2; ++k) {
+        float2 v = unpack<T>(xw[k]), w = unpack<T>(yw[k]);
+        turn_pair(v.x, w.x, c[2 * k], s[2 * k]);
+        turn_pair(v.y, w.y, c[2 * k + 1], s[2 * k + 1]);
+        xw[k] = pack<T>(v.x, v.y);
+        yw[k] = pack<T>(w.x, w.y);
+      }
+    }
   }
 }
 
@@ -120,8 +158,8 @@ struct Share {
   int lanes, rows;
   int token_first;  // neighbours take the next token, not the next lane
 };
-constexpr int kFlight = 2;  // rows whose loads a thread has under way at once
 constexpr int kRows = 4;    // most rows of a thread
+constexpr int kFlight = 2;  // rows whose loads a thread has under way at once
 
 struct Place {
   long long token;
@@ -151,17 +189,18 @@ __device__ __forceinline__ Place place_of(long long index, const RowShape& r, co
 // Moves one item of a thread's rows. `source(i)` gives the i-th row, or null;
 // `ready` looks up what `target(i)` (null: drop the row) and the cosines need,
 // while the first rows are on their way.
-template <typename T, int P, class Source, class Ready, class Target, class Turns>
+template <typename T, int P, bool ROTATES, class Source, class Ready, class Target, class Turns>
 __device__ __forceinline__ void move_rows(const RowShape& s, int item, int rows, Source source, Ready ready,
                                           Target target, Turns turns) {
   using U = Unit<T, P>;
   int u0, u1;
   bool two;
   item_offsets<P>(s, item, u0, u1, two);
-  U x[kFlight], y[kFlight];
+  constexpr int N = kFlight;
+  U x[N], y[N];
   auto load = [&](int i0) {
 #pragma unroll
-    for (int i = 0; i < kFlight; ++i) {
+    for (int i = 0; i < N; ++i) {
       const T* src = i0 + i < rows ? source(i0 + i) : nullptr;
       if (src) {
         x[i] = *reinterpret_cast<const U*>(src + u0);
@@ -172,13 +211,13 @@ __device__ __forceinline__ void move_rows(const RowShape& s, int item, int rows,
   load(0);
   float c[P], sn[P];
   if (!ready(c, sn)) return;
-  for (int i0 = 0; i0 < rows; i0 += kFlight) {
+  for (int i0 = 0; i0 < rows; i0 += N) {
     if (i0) load(i0);
 #pragma unroll
-    for (int i = 0; i < kFlight; ++i) {
+    for (int i = 0; i < N; ++i) {
       T* dst = i0 + i < rows ? target(i0 + i) : nullptr;
       if (dst) {
-        if (turns(i0 + i)) turn<T, P>(x[i], y[i], c, sn, s.interleaved != 0);
+        if (ROTATES && turns(i0 + i)) turn<T, P>(x[i], y[i], c, sn, s.interleaved != 0);
         *reinterpret_cast<U*>(dst + u0) = x[i];
         if (two) *reinterpret_cast<U*>(dst + u1) = y[i];
       }
@@ -212,11 +251,11 @@ __global__ void __launch_bounds__(256, 4) rope_kernel(const RopeParams p) {
   T* dst = static_cast<T*>(p.y) + b * p.ys_b + at.token * p.ys_s + at.lane * p.ys_h;
   const bool rotated = at.item < p.row.rot_items;
   const int rows = min(p.share.rows, (p.H - at.lane + p.share.lanes - 1) / p.share.lanes);
-  move_rows<T, P>(
+  move_rows<T, P, true>(
       p.row, at.item, rows, [&](int i) { return src + i * p.share.lanes * p.xs_h; },
       [&](float(&c)[P], float(&s)[P]) {
         if (rotated)
-          angles<P>(p.inv_freq + at.item * P, p.positions[b * p.pos_stride_b + at.token], p.factor,
+          angles<T, P>(p.inv_freq + at.item * P, p.positions[b * p.pos_stride_b + at.token], p.factor,
                     p.backward != 0, c, s);
         return true;
       },
@@ -241,18 +280,18 @@ struct AppendParams {
 };
 
 // grid: x over the shares; the q, k and v heads of a token are numbered through.
-template <typename T, int P>
-__global__ void __launch_bounds__(256, 4) paged_append_kernel(const AppendParams p) {
+template <typename T, int P, bool ROTATES>
+__global__ void __launch_bounds__(256, ROTATES ? 4 : 6) paged_append_kernel(const AppendParams p) {
   const long long index = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
   if (index >= static_cast<long long>(p.T) * p.share.lanes * p.row.items) return;
   const Place at = place_of(index, p.row, p.share, p.T);
   const long long token = at.token;
   const int all = p.Hq + 2 * p.Hkv;
   const int rows = min(p.share.rows, (all - at.lane + p.share.lanes - 1) / p.share.lanes);
-  const bool rotated = at.item < p.row.rot_items;
+  const bool rotated = ROTATES && at.item < p.row.rot_items;
   auto head = [&](int i) { return at.lane + i * p.share.lanes; };
   T *k_row = nullptr, *v_row = nullptr;  // this token's row of head 0 in the pools, null to drop it
-  move_rows<T, P>(
+  move_rows<T, P, ROTATES>(
       p.row, at.item, rows,
       [&](int i) {
         const int h = head(i);
@@ -269,8 +308,9 @@ __global__ void __launch_bounds__(256, 4) paged_append_kernel(const AppendParams
           if (where == paged::kMisplaced) atomicCAS(p.err, 0, kErrBadBatch);
           return false;
         }
-        long long slot = position / p.page_size;
-        const int row = static_cast<int>(position - slot * p.page_size);
+        const unsigned at32 = static_cast<unsigned>(position);  // lengths have 31 bits
+        const int slot = at32 / static_cast<unsigned>(p.page_size);
+        const int row = at32 - slot * p.page_size;
         const int page = slot < p.table_width
                              ? paged::clip_page(__ldg(p.page_table + seq * p.table_stride + slot), p.num_pages)
                              : p.num_pages;
@@ -280,7 +320,7 @@ __global__ void __launch_bounds__(256, 4) paged_append_kernel(const AppendParams
         } else {
           atomicCAS(p.err, 0, kErrBadBatch);
         }
-        if (rotated) angles<P>(p.inv_freq + at.item * P, position, p.factor, false, c, s);
+        if (rotated) angles<T, P>(p.inv_freq + at.item * P, position, p.factor, false, c, s);
         return true;
       },
       [&](int i) -> T* {
