@@ -131,7 +131,8 @@ Plan make_plan(const pkb200_paged_cache* c, const pkb200_paged_batch* b, int q_h
     return o;
   };
   if (pl.rows_mr) {
-    pl.rows_grid = sms * (pl.dp <= 128 ? 2 : 1);
+    pl.rows_grid = sms * (pl.dp == 64 ? paged::RowsCfg<64, 16>::kBlocks : pl.dp == 128 ? paged::RowsCfg<128, 16>::kBlocks
+                                                                        : paged::RowsCfg<256, 16>::kBlocks);
     const size_t slots = 2 * static_cast<size_t>(pl.rows_grid) + 2;
     pl.rows_o = take(slots * pl.rows_mr * pl.dp * 4);
     pl.rows_ml = take(slots * pl.rows_mr * 8);
@@ -196,9 +197,9 @@ int box_for(int page_size, int most) {
 
 // Launches the joining pass so that it may start while the attention kernel drains.
 template <typename T, int DP>
-int launch_join(const paged::AttnParams& a, int entries, int slot_rows, cudaStream_t s) {
+int launch_join(const paged::AttnParams& a, int entries, int slot_rows, int block_rows, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(entries, (slot_rows + 3) / 4);
+  cfg.gridDim = dim3(entries, slot_rows / block_rows);
   cfg.blockDim = dim3(paged::kJoinThreads);
   cfg.stream = s;
   cudaLaunchAttribute early;
@@ -206,7 +207,7 @@ int launch_join(const paged::AttnParams& a, int entries, int slot_rows, cudaStre
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged::paged_join_kernel<T, DP>, a, slot_rows);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged::paged_join_kernel<T, DP>, a, slot_rows, block_rows);
   internal::count_launch(internal::kOther);
   return e;
 }
@@ -229,7 +230,7 @@ int launch_rows(const pkb200_paged_cache* c, paged::AttnParams a, const Plan& pl
   kernel<<<pl.rows_grid, C::kThreads, C::SMEM, s>>>(mk, mv, a);
   internal::count_launch(internal::kOther);
   if (const int e = cudaGetLastError()) return e;
-  return launch_join<T, DP>(a, pl.rows_grid, MR, s);
+  return launch_join<T, DP>(a, pl.rows_grid, MR, MR / 4, s);
 }
 
 template <typename T, int DP>
@@ -265,7 +266,7 @@ int launch_tiles(const pkb200_paged_cache* c, paged::AttnParams a, const Plan& p
   kernel<<<static_cast<unsigned>(entries * pl.splits), C::kThreads, C::SMEM, s>>>(mq, mk, mv, a);
   internal::count_launch(internal::kAttnTensor);
   if (const int e = cudaGetLastError()) return e;
-  return pl.splits > 1 ? launch_join<T, DP>(a, static_cast<int>(entries), 256, s) : 0;
+  return pl.splits > 1 ? launch_join<T, DP>(a, static_cast<int>(entries), 256, 16, s) : 0;
 }
 
 template <typename T, int DP>

@@ -106,6 +106,8 @@ __device__ __forceinline__ uint32_t not_finite4(const uint4& w) {
   return t & 0x80008000u;
 }
 
+constexpr float kStaleMax = 8.f;  // log2 units a row's maximum may lag behind
+
 // Weight of a part whose maximum is m within a row whose maximum is top.
 __device__ __forceinline__ float part_weight(float m, float top) {
   return m == top ? 1.f : fast_exp2(m - top);
@@ -141,27 +143,25 @@ __device__ __forceinline__ long long block_prefix(long long mine, long long* war
 }
 
 // ------------------------------------------------------------------- join --
-// Adds up the pieces of row tiles whose keys several blocks went over: 4 rows
-// per block, 4 warps to a row, each taking every fourth piece. The order of the
-// sums is fixed, so results do not depend on timing. Launched to overlap the
-// attention kernel's tail (grid_dependency_wait).
-constexpr int kJoinThreads = 512;
+// Adds up the pieces of row tiles whose keys several blocks went over, `rows`
+// rows per block. A row with few pieces is one warp's; with many, four warps
+// share it, each taking every fourth piece. The order of the sums is fixed, so results do not depend on timing.
+// Launched to overlap the attention kernel's tail (grid_dependency_wait).
+constexpr int kJoinThreads = 512, kJoinFew = 8;
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttnParams p, int slot_rows) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttnParams p, int slot_rows,
+                                                                  int block_rows) {
   constexpr int C = (DP + 127) / 128;  // float4 per lane
   __shared__ float4 o_s[3][4][32 * C];
   __shared__ float2 ml_s[3][4];
   grid_dependency_wait();
   const Entry e = reinterpret_cast<const Entry*>(p.meta)[blockIdx.x];
+  const int first = static_cast<int>(blockIdx.y) * block_rows, end = min(first + block_rows, e.rows);
+  if (e.pieces == 0 || first >= end) return;
   const int warp = warp_id(), lane = lane_id();
-  const int row = static_cast<int>(blockIdx.y) * 4 + (warp & 3);
-  const int part = warp >> 2;
-  if (e.pieces == 0 || static_cast<int>(blockIdx.y) * 4 >= e.rows) return;
-  float m = -INFINITY, l = 0.f;
+  float m, l;
   float4 o[C];
-#pragma unroll
-  for (int c = 0; c < C; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](float mk, float lk, const float4 (&ok)[C]) {
     const float top = fmaxf(m, mk);
     const float a = part_weight(m, top), b = part_weight(mk, top);
@@ -175,9 +175,13 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttnPara
       o[c].w = o[c].w * a + ok[c].w * b;
     }
   };
-  if (row < e.rows) {
+  auto gather = [&](int row, int from, int step) {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int k = part; k < e.pieces; k += 4) {
+    for (int k = from; k < e.pieces; k += step) {
       const long long at = static_cast<long long>(k == 0 ? e.slot0 : e.slot1 + (k - 1) * e.step) * slot_rows + row;
       const float2 ml = p.part_ml[at];
       float4 ok[C];
@@ -189,34 +193,50 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttnPara
       }
       add(ml.x, ml.y, ok);
     }
-  }
-  if (part > 0) {
+  };
+  auto store = [&](int row) {
+    const int r = e.row0 + row, tr = r / p.G, h = e.hk * p.G + r - tr * p.G;
+    const long long t = e.t0 + tr;
+    const float inv = inverse_sum(l);
+    T* dst = static_cast<T*>(p.out) + t * p.os_t + h * p.os_h;
 #pragma unroll
-    for (int c = 0; c < C; ++c) o_s[part - 1][warp & 3][c * 32 + lane] = o[c];
-    if (lane == 0) ml_s[part - 1][warp & 3] = make_float2(m, l);
+    for (int c = 0; c < C; ++c) {
+      const int d = lane * 4 + c * 128;
+      if (d < p.D)
+        *reinterpret_cast<uint2*>(dst + d) =
+            make_uint2(pack2<T>(o[c].x * inv, o[c].y * inv), pack2<T>(o[c].z * inv, o[c].w * inv));
+    }
+    if (p.lse && lane == 0) p.lse[t * p.Hq + h] = log_sum(m, l);
+  };
+  if (e.pieces <= kJoinFew) {
+    for (int row = first + warp; row < end; row += kJoinThreads / 32) {
+      gather(row, 0, 1);
+      store(row);
+    }
+    return;
   }
-  __syncthreads();
-  if (part > 0 || row >= e.rows) return;
-  for (int w = 0; w < 3; ++w) {
-    float4 ok[C];
+  const int part = warp >> 2, mine = warp & 3;
+  for (int row0 = first; row0 < end; row0 += 4) {
+    const int row = row0 + mine;
+    if (row < end) gather(row, part, 4);
+    if (part > 0 && row < end) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) ok[c] = o_s[w][warp][c * 32 + lane];
-    const float2 ml = ml_s[w][warp];
-    add(ml.x, ml.y, ok);
-  }
-  const int r = e.row0 + row;
-  const long long t = e.t0 + r / p.G;
-  const int h = e.hk * p.G + r % p.G;
-  const float inv = inverse_sum(l);
-  T* dst = static_cast<T*>(p.out) + t * p.os_t + h * p.os_h;
+      for (int c = 0; c < C; ++c) o_s[part - 1][mine][c * 32 + lane] = o[c];
+      if (lane == 0) ml_s[part - 1][mine] = make_float2(m, l);
+    }
+    __syncthreads();
+    if (part == 0 && row < end) {
+      for (int w = 0; w < 3; ++w) {
+        float4 ok[C];
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int d = lane * 4 + c * 128;
-    if (d < p.D)
-      *reinterpret_cast<uint2*>(dst + d) =
-          make_uint2(pack2<T>(o[c].x * inv, o[c].y * inv), pack2<T>(o[c].z * inv, o[c].w * inv));
+        for (int c = 0; c < C; ++c) ok[c] = o_s[w][mine][c * 32 + lane];
+        const float2 ml = ml_s[w][mine];
+        add(ml.x, ml.y, ok);
+      }
+      store(row);
+    }
+    __syncthreads();
   }
-  if (p.lse && lane == 0) p.lse[t * p.Hq + h] = log_sum(m, l);
 }
 
 }  // namespace paged

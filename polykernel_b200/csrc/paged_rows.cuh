@@ -14,9 +14,11 @@
 // 7/8 empty, and the tensor work is a small part of the time of the reads).
 // With MR = 16 rows each warp takes 16 of a tile's 64 keys with statistics of
 // its own, merged at the end of the row tile; with MR = 32 or 64 two or all
-// four warps take different rows. P enters the P.V product as two 16-bit terms
-// (value and remainder), so the output carries no rounding of P: the second
-// product costs nothing that the reads do not hide.
+// four warps take different rows. Up to 32 rows P enters the P.V product as two
+// 16-bit terms (value and remainder), so the output carries no rounding of P:
+// the second product costs nothing that the reads do not hide. With 64 rows the
+// tensor work (8 cycles per mma.sync and sub-partition) comes near the time of the
+// reads, and P is rounded once to the inputs' type, as in the tile kernel.
 #pragma once
 
 #include "paged_common.cuh"
@@ -30,27 +32,30 @@ struct RowsCfg {
   static constexpr int kThreads = 160;  // 4 compute warps, 1 that fetches
   static constexpr int WM = MR / 16, WK = 4 / WM, KW = KT / WK;  // warps by rows and by keys
   static constexpr int SLOT = KT * DP * 2;
-  // 80 KB in flight per block, two blocks per SM (one with 256-wide heads)
+  static constexpr bool kSplitP = MR <= 32;
+  // Blocks per SM, as many as their registers allow: the work on a tile is a
+  // chain of short steps. 130 to 150 KB per SM are in flight.
   static constexpr int kBlocks = DP <= 128 ? 2 : 1;
-  static constexpr int SLOTS = DP == 64 ? 10 : DP == 128 ? 5 : 5;
-  static constexpr int OFF_STAGE = SLOTS * SLOT;  // merge: 2 x 16 rows of fp32
-  static constexpr int STAGE = WK > 1 ? 2 * 16 * DP * 4 : 0;
-  static constexpr int OFF_ML = OFF_STAGE + STAGE;        // float2[4][16]
-  static constexpr int OFF_BAR = OFF_ML + 4 * 16 * 8;     // full[SLOTS], empty[SLOTS]
-  static constexpr int OFF_SCAN = OFF_BAR + 2 * SLOTS * 8;  // long long[5], start of the run
+  static constexpr int SLOTS = DP == 64 ? 10 : 4;
+  // Merge: each warp's 16 rows of fp32, rows 32 bytes apart in the banks
+  static constexpr int STRIDE = DP + 8;
+  static constexpr int OFF_STAGE = SLOTS * SLOT;
+  static constexpr int OFF_ML = OFF_STAGE + 4 * 16 * STRIDE * 4;  // float2[4][16]
+  static constexpr int OFF_BAR = OFF_ML + 4 * 16 * 8;             // full[SLOTS], empty[SLOTS]
+  static constexpr int OFF_SCAN = OFF_BAR + 2 * SLOTS * 8;        // long long[5], start of the run
   static constexpr int SMEM = OFF_SCAN + 5 * 8 + 32 + 1024;
 };
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, __half>::value)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
         "{%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
         "{%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -59,16 +64,22 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
+               : "r"(addr));
 }
 __device__ __forceinline__ void compute_warps_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+constexpr int kAhead = 3;  // steps between the load of a fragment and its products
+
+// 64-bit division is a long subroutine; most counts fit 32 bits.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
 
 // Place in the line of work: a row tile `rt` of key head `hk` of sequence `b`.
 template <int MR>
@@ -85,6 +96,7 @@ struct RowCursor {
     return rows >= p.min_rows && rows <= p.max_rows ? rows : 0;
   }
   __device__ static int tiles_of(const AttnParams& p, const Seq& s, int rows, int rt, int& tile0) {
+    if (rows <= MR) return key_tiles<64>(p, s, 0, s.nq - 1, tile0);
     return key_tiles<64>(p, s, rt * MR / p.G, (min(rows, rt * MR + MR) - 1) / p.G, tile0);
   }
   // Key tiles of a whole sequence (one key head).
@@ -106,7 +118,7 @@ struct RowCursor {
     b = b_;
     load();
     const long long per_head = units_of(p, s);
-    hk = static_cast<int>(rem / per_head);
+    hk = static_cast<int>(divide(rem, per_head));
     rem -= hk * per_head;
     for (rt = 0;; ++rt) {
       n = tiles_of(p, s, rows, rt, tile0);
@@ -166,7 +178,7 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
     for (int b = b0; b < b1; ++b) mine += p.Hkv * RowCursor<MR>::units_of(p, load_seq(p, b, true));
     long long total;
     const long long before = block_prefix<C::kThreads>(mine, scan, total);
-    per_block = max(static_cast<long long>(p.min_units), (total + gridDim.x - 1) / gridDim.x);
+    per_block = max(static_cast<long long>(p.min_units), divide(total + gridDim.x - 1, gridDim.x));
     u0 = blockIdx.x * per_block;
     u1 = min(total, u0 + per_block);
     if (u0 >= u1) {
@@ -300,16 +312,21 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
       if (!ok) break;
       {
         const uint32_t base = slots_addr + slot * C::SLOT;
+        // fragments are loaded kAhead steps before the products that use them
+        uint32_t kf[kAhead + 1][4];
+        auto load = [&](int i) {
+          const int ks = i / (KW / 16), key = key_k + i % (KW / 16) * 16, c = (ks & 3) * 2 + chunk_k;
+          ldmatrix4(base + (ks >> 2) * (KT * 128) + key * 128 + ((c ^ (key & 7)) << 4), kf[i % (kAhead + 1)]);
+        };
+        constexpr int N = DP / 16 * (KW / 16);
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
+        for (int i = 0; i < kAhead; ++i) load(i);
 #pragma unroll
-          for (int n = 0; n < KW / 16; ++n) {
-            const int key = key_k + n * 16, c = (ks & 3) * 2 + chunk_k;
-            uint32_t kf[4];
-            ldmatrix4(base + (ks >> 2) * (KT * 128) + key * 128 + ((c ^ (key & 7)) << 4), kf);
-            mma16816<T>(s[2 * n], qf[ks], kf[0], kf[1]);
-            mma16816<T>(s[2 * n + 1], qf[ks], kf[2], kf[3]);
-          }
+        for (int i = 0; i < N; ++i) {
+          if (i + kAhead < N) load(i + kAhead);
+          const int ks = i / (KW / 16), n = i % (KW / 16), f = i % (kAhead + 1);
+          mma16816<T>(s[2 * n], qf[ks], kf[f][0], kf[f][1]);
+          mma16816<T>(s[2 * n + 1], qf[ks], kf[f][2], kf[f][3]);
         }
       }
       __syncwarp();
@@ -331,19 +348,23 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
           }
         }
       }
-      float mx_a = -INFINITY, mx_b = -INFINITY;
+      float mx_a = fmaxf(s[0][0], s[0][1]), mx_b = fmaxf(s[0][2], s[0][3]);
 #pragma unroll
-      for (int n = 0; n < KW / 8; ++n) {
-        mx_a = fmaxf(mx_a, fmaxf(s[n][0], s[n][1]));
-        mx_b = fmaxf(mx_b, fmaxf(s[n][2], s[n][3]));
+      for (int n = 1; n < KW / 8; ++n) {
+        mx_a = fmax3(mx_a, s[n][0], s[n][1]);
+        mx_b = fmax3(mx_b, s[n][2], s[n][3]);
       }
+      // The running maximum moves only when a score passes it by 2^8 (P stays
+      // below 2^8; P and the sums share the stale maximum, so the quotient is
+      // exact): after a row's first tiles that is rare, and one vote rules it out.
+      if (__any_sync(0xffffffffu, fmaf(mx_a, p.scale_log2, -kStaleMax) > m_a ||
+                                      fmaf(mx_b, p.scale_log2, -kStaleMax) > m_b)) {
 #pragma unroll
-      for (int x = 1; x <= 2; x <<= 1) {
-        mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, x));
-        mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, x));
-      }
-      const float new_a = fmaxf(m_a, mx_a * p.scale_log2), new_b = fmaxf(m_b, mx_b * p.scale_log2);
-      if (__any_sync(0xffffffffu, new_a != m_a || new_b != m_b)) {
+        for (int x = 1; x <= 2; x <<= 1) {
+          mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, x));
+          mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, x));
+        }
+        const float new_a = fmaxf(m_a, mx_a * p.scale_log2), new_b = fmaxf(m_b, mx_b * p.scale_log2);
         const float fa = part_weight(m_a, new_a), fb = part_weight(m_b, new_b);
         m_a = new_a;
         m_b = new_b;
@@ -357,15 +378,25 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
           o[d][3] *= fb;
         }
       }
-      const float sub_a = m_a == -INFINITY ? 0.f : m_a, sub_b = m_b == -INFINITY ? 0.f : m_b;
+      {
+        const float sub_a = m_a == -INFINITY ? 0.f : -m_a, sub_b = m_b == -INFINITY ? 0.f : -m_b;
+        const uint64_t sc2 = f2_pack(p.scale_log2, p.scale_log2);
+        const uint64_t a2 = f2_pack(sub_a, sub_a), b2 = f2_pack(sub_b, sub_b);
+        uint64_t la2 = f2_pack(l_a, 0.f), lb2 = f2_pack(l_b, 0.f);
 #pragma unroll
-      for (int n = 0; n < KW / 8; ++n) {
-        s[n][0] = fast_exp2(fmaf(s[n][0], p.scale_log2, -sub_a));
-        s[n][1] = fast_exp2(fmaf(s[n][1], p.scale_log2, -sub_a));
-        s[n][2] = fast_exp2(fmaf(s[n][2], p.scale_log2, -sub_b));
-        s[n][3] = fast_exp2(fmaf(s[n][3], p.scale_log2, -sub_b));
-        l_a += s[n][0] + s[n][1];
-        l_b += s[n][2] + s[n][3];
+        for (int n = 0; n < KW / 8; ++n) {
+          f2_unpack(f2_fma(f2_pack(s[n][0], s[n][1]), sc2, a2), s[n][0], s[n][1]);
+          f2_unpack(f2_fma(f2_pack(s[n][2], s[n][3]), sc2, b2), s[n][2], s[n][3]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[n][c] = fast_exp2(s[n][c]);
+          la2 = f2_add(la2, f2_pack(s[n][0], s[n][1]));
+          lb2 = f2_add(lb2, f2_pack(s[n][2], s[n][3]));
+        }
+        float x, y;
+        f2_unpack(la2, x, y);
+        l_a = x + y;
+        f2_unpack(lb2, x, y);
+        l_b = x + y;
       }
       // ---- O += P V
       ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], parity, p.err, abort_flag, kErrTimeoutSoftmax));
@@ -390,6 +421,14 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
         by_hand = __any_sync(0xffffffffu, bad);
       }
       if (!by_hand) {
+        uint32_t vf[kAhead + 1][4];
+        auto load = [&](int i) {
+          const int d = i % (DP / 16), key = key_v + i / (DP / 16) * 16, c = (d & 3) * 2 + chunk_v;
+          ldmatrix4_trans(base + (d >> 2) * (KT * 128) + key * 128 + ((c ^ (key & 7)) << 4), vf[i % (kAhead + 1)]);
+        };
+        constexpr int N = KW / 16 * (DP / 16);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) load(i);
 #pragma unroll
         for (int kb = 0; kb < KW / 16; ++kb) {
           uint32_t ph[4], pl[4];
@@ -397,18 +436,21 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
           for (int x = 0; x < 4; ++x) {
             const float v0 = s[2 * kb + (x >> 1)][(x & 1) * 2], v1 = s[2 * kb + (x >> 1)][(x & 1) * 2 + 1];
             ph[x] = pack2<T>(v0, v1);
-            const float2 r = unpack2<T>(ph[x]);
-            pl[x] = pack2<T>(v0 - r.x, v1 - r.y);
+            if constexpr (C::kSplitP) {
+              const float2 r = unpack2<T>(ph[x]);
+              pl[x] = pack2<T>(v0 - r.x, v1 - r.y);
+            }
           }
 #pragma unroll
           for (int d = 0; d < DP / 16; ++d) {
-            const int key = key_v + kb * 16, c = (d & 3) * 2 + chunk_v;
-            uint32_t vf[4];
-            ldmatrix4_trans(base + (d >> 2) * (KT * 128) + key * 128 + ((c ^ (key & 7)) << 4), vf);
-            mma16816<T>(o[2 * d], ph, vf[0], vf[1]);
-            mma16816<T>(o[2 * d + 1], ph, vf[2], vf[3]);
-            mma16816<T>(o[2 * d], pl, vf[0], vf[1]);
-            mma16816<T>(o[2 * d + 1], pl, vf[2], vf[3]);
+            const int i = kb * (DP / 16) + d, f = i % (kAhead + 1);
+            if (i + kAhead < N) load(i + kAhead);
+            mma16816<T>(o[2 * d], ph, vf[f][0], vf[f][1]);
+            mma16816<T>(o[2 * d + 1], ph, vf[f][2], vf[f][3]);
+            if constexpr (C::kSplitP) {
+              mma16816<T>(o[2 * d], pl, vf[f][0], vf[f][1]);
+              mma16816<T>(o[2 * d + 1], pl, vf[f][2], vf[f][3]);
+            }
           }
         }
       } else {
@@ -451,107 +493,71 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
     }
     if (!ok) break;
 
-    // ---- merge the warps that took the same rows' keys
+    // ---- join the warps that took the same rows' keys, through shared memory;
+    // rows leave as whole lines: the output, or a piece for the joining pass
 #pragma unroll
     for (int x = 1; x <= 2; x <<= 1) {
       l_a += __shfl_xor_sync(0xffffffffu, l_a, x);
       l_b += __shfl_xor_sync(0xffffffffu, l_b, x);
     }
-    if constexpr (WK > 1) {
+    {
+      float* own = stage + warp * 16 * C::STRIDE;
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d) {
+        *reinterpret_cast<float2*>(own + g * C::STRIDE + d * 8 + t4 * 2) = make_float2(o[d][0], o[d][1]);
+        *reinterpret_cast<float2*>(own + (g + 8) * C::STRIDE + d * 8 + t4 * 2) = make_float2(o[d][2], o[d][3]);
+      }
       if (t4 == 0) {
         ml_s[warp * 16 + g] = make_float2(m_a, l_a);
         ml_s[warp * 16 + g + 8] = make_float2(m_b, l_b);
       }
-      compute_warps_sync();
-      float top_a = -INFINITY, top_b = -INFINITY, sum_a = 0.f, sum_b = 0.f;
-#pragma unroll
-      for (int w = 0; w < WK; ++w) {
-        top_a = fmaxf(top_a, ml_s[(wm * WK + w) * 16 + g].x);
-        top_b = fmaxf(top_b, ml_s[(wm * WK + w) * 16 + g + 8].x);
-      }
-#pragma unroll
-      for (int w = 0; w < WK; ++w) {
-        const float2 xa = ml_s[(wm * WK + w) * 16 + g], xb = ml_s[(wm * WK + w) * 16 + g + 8];
-        sum_a += xa.y * part_weight(xa.x, top_a);
-        sum_b += xb.y * part_weight(xb.x, top_b);
-      }
-      const float fa = part_weight(m_a, top_a), fb = part_weight(m_b, top_b);
-      m_a = top_a;
-      m_b = top_b;
-      l_a = sum_a;
-      l_b = sum_b;
-#pragma unroll
-      for (int d = 0; d < DP / 8; ++d) {
-        o[d][0] *= fa;
-        o[d][1] *= fa;
-        o[d][2] *= fb;
-        o[d][3] *= fb;
-      }
-#pragma unroll
-      for (int left = WK / 2; left >= 1; left >>= 1) {
-        float* buf = stage + (wm * (WK / 2) + (wk & (left - 1))) * 16 * DP;
-        if (wk >= left && wk < 2 * left) {
-#pragma unroll
-          for (int d = 0; d < DP / 8; ++d) {
-            *reinterpret_cast<float2*>(buf + g * DP + d * 8 + t4 * 2) = make_float2(o[d][0], o[d][1]);
-            *reinterpret_cast<float2*>(buf + (g + 8) * DP + d * 8 + t4 * 2) = make_float2(o[d][2], o[d][3]);
-          }
-        }
-        compute_warps_sync();
-        if (wk < left) {
-#pragma unroll
-          for (int d = 0; d < DP / 8; ++d) {
-            const float2 xa = *reinterpret_cast<float2*>(buf + g * DP + d * 8 + t4 * 2);
-            const float2 xb = *reinterpret_cast<float2*>(buf + (g + 8) * DP + d * 8 + t4 * 2);
-            o[d][0] += xa.x;
-            o[d][1] += xa.y;
-            o[d][2] += xb.x;
-            o[d][3] += xb.y;
-          }
-        }
-        if (left > 1) compute_warps_sync();
-      }
     }
-    // ---- output, or a piece for the joining pass
+    compute_warps_sync();
     const bool begins = off == 0, ends = off + run == at.n;
-    if (wk == 0) {
-      if (begins && ends) {
-        const float ia = inverse_sum(l_a), ib = inverse_sum(l_b);
+    const bool whole = begins && ends;
+    const long long slot_row = (2LL * blockIdx.x + (begins ? 1 : 0)) * MR;
+    constexpr int ACROSS = DP / 4;  // threads of a row, four values each
+    const int col = static_cast<int>(threadIdx.x) % ACROSS * 4;
+#pragma unroll 1
+    for (int r = static_cast<int>(threadIdx.x) / ACROSS; r < MR; r += 128 / ACROSS) {
+      const int seq_row = at.rt * MR + r;
+      if (seq_row >= at.rows) break;
+      const float2* ml = ml_s + (r / 16) * WK * 16 + r % 16;
+      float m = ml[0].x;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int r = row0 + g + half * 8;
-          if (r < at.rows) {
-            const long long t = at.s.t0 + r / p.G;
-            const int h = at.hk * p.G + r % p.G;
-            T* dst = static_cast<T*>(p.out) + t * p.os_t + h * p.os_h;
-            const float inv = half ? ib : ia;
+      for (int w = 1; w < WK; ++w) m = fmaxf(m, ml[w * 16].x);
+      float l = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int d = 0; d < DP / 8; ++d)
-              if (d * 8 < p.D)
-                *reinterpret_cast<uint32_t*>(dst + d * 8 + t4 * 2) =
-                    pack2<T>(o[d][half * 2] * inv, o[d][half * 2 + 1] * inv);
-            if (p.lse && t4 == 0)
-              p.lse[t * p.Hq + h] = log_sum(half ? m_b : m_a, half ? l_b : l_a);
-          }
-        }
+      for (int w = 0; w < WK; ++w) {
+        const float2 part = ml[w * 16];
+        const float f = part_weight(part.x, m);
+        const float4 x = *reinterpret_cast<const float4*>(stage + (((r / 16) * WK + w) * 16 + r % 16) * C::STRIDE + col);
+        l = fmaf(part.y, f, l);
+        v.x = fmaf(x.x, f, v.x);
+        v.y = fmaf(x.y, f, v.y);
+        v.z = fmaf(x.z, f, v.z);
+        v.w = fmaf(x.w, f, v.w);
+      }
+      if (whole) {
+        const int tr = seq_row / p.G, h = at.hk * p.G + seq_row - tr * p.G;
+        const long long t = at.s.t0 + tr;
+        const float inv = inverse_sum(l);
+        if (col < p.D)
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + t * p.os_t + h * p.os_h + col) =
+              make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+        if (p.lse && col == 0) p.lse[t * p.Hq + h] = log_sum(m, l);
       } else {
-        const long long slot_row = (2LL * blockIdx.x + (begins ? 1 : 0)) * MR + wm * 16;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          float* dst = p.part_o + (slot_row + g + half * 8) * DP;
-#pragma unroll
-          for (int d = 0; d < DP / 8; ++d)
-            *reinterpret_cast<float2*>(dst + d * 8 + t4 * 2) = make_float2(o[d][half * 2], o[d][half * 2 + 1]);
-          if (t4 == 0)
-            p.part_ml[slot_row + g + half * 8] = half ? make_float2(m_b, l_b) : make_float2(m_a, l_a);
-        }
+        *reinterpret_cast<float4*>(p.part_o + (slot_row + r) * DP + col) = v;
+        if (col == 0) p.part_ml[slot_row + r] = make_float2(m, l);
       }
     }
+    compute_warps_sync();  // the stage is free again
     if (begins && !ends) {  // only ever the run's last row tile
       wrote_meta = true;
       if (threadIdx.x == 0) {
         Entry e;
-        e.pieces = static_cast<int>((u + at.n - 1) / per_block - blockIdx.x) + 1;
+        e.pieces = static_cast<int>(divide(u + at.n - 1, per_block) - blockIdx.x) + 1;
         e.t0 = at.s.t0;
         e.hk = at.hk;
         e.row0 = at.rt * MR;

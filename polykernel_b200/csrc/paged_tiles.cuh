@@ -55,7 +55,6 @@ struct TilesCfg {
   static_assert(2 * kRegsSoftmax + kRegsValues + kRegsControl == 4 * 128, "launch: 512 x 128");
   static_assert(SMEM <= 232448, "shared memory of an SM");
 };
-constexpr float kStaleMax = 8.f;  // log2 units a row's maximum may lag behind
 
 // One item of work, as the work warp hands it to the others.
 struct alignas(64) TileWork {
