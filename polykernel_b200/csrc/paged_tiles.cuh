@@ -5,9 +5,10 @@
 // 2048 cycles of tensor work per 128-key tile at head width 128, and their 2 x
 // 128 x 128 exponentials cost the same at 16 a cycle. So a block works on two
 // 128-row tiles (A, B) that share every key tile: while the tensor cores form
-// P.V and the next S of one, a warpgroup takes the softmax of the other; and a
-// part of the exponentials is formed on the FMA pipe. Rows are the G heads of
-// consecutive tokens, so a key tile is fetched once for the group.
+// P.V and the next S of one, a warpgroup takes the softmax of the other. Rows are
+// the G heads of consecutive tokens, so a key tile is fetched once for the group.
+// Long runs are under the power cap: a quarter of the exponentials formed on the
+// FMA pipe instead took as many cycles and 3% more time, at a lower clock.
 //   warps 0-3, 4-7   softmax of A and of B: thread r owns row r (TMEM lane r),
 //                    reads its 128 scores, writes P back over them as 16-bit
 //                    pairs (the A operand of P.V), rescales O in TMEM when the
@@ -56,6 +57,8 @@ struct TilesCfg {
   static_assert(SMEM <= 232448, "shared memory of an SM");
 };
 
+constexpr int kEarly = 2;  // quarters of a tile's keys whose P is handed over ahead of the rest
+
 // One item of work, as the work warp hands it to the others.
 struct alignas(64) TileWork {
   int b;              // sequence; -1: no more items
@@ -67,39 +70,6 @@ struct alignas(64) TileWork {
   int by_hand;        // values of masked keys are not finite
 };
 static_assert(sizeof(TileWork) == 64, "");
-
-// 2^x of a pair on the FMA and integer pipes, for x >= -126; values from -127
-// down (and -inf) give 0. The SFU takes 8 cycles for a warp's ex2, which would
-// bound the softmax alone. x = n + f with n whole and |f| <= 1/2 (adding 1.5 *
-// 2^23 rounds to whole numbers and leaves n in the low bits); 2^f = 1 + f (c1 +
-// ...), the degree-4 polynomial of that form with the least relative error on
-// the interval (iterated weighted least squares: 2.9e-6, below the rounding of
-// P); n goes into the exponent. NaN is not carried through.
-__device__ __forceinline__ void exp2_pair(uint64_t x2, float& e0, float& e1) {
-  constexpr float kRound = 12582912.f;  // 1.5 * 2^23
-  constexpr float c1 = 0.69312418f, c2 = 0.24024099f, c3 = 0.055906426f, c4 = 0.009582853f;
-  float x0, x1;
-  f2_unpack(x2, x0, x1);
-  x2 = f2_pack(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
-  const uint64_t t2 = f2_add(x2, f2_pack(kRound, kRound));
-  const uint64_t f2 = f2_sub(x2, f2_sub(t2, f2_pack(kRound, kRound)));
-  uint64_t p2 = f2_fma(f2_pack(c4, c4), f2, f2_pack(c3, c3));
-  p2 = f2_fma(p2, f2, f2_pack(c2, c2));
-  p2 = f2_fma(p2, f2, f2_pack(c1, c1));
-  p2 = f2_fma(p2, f2, f2_pack(1.f, 1.f));
-  float t0, t1, p0, p1;
-  f2_unpack(t2, t0, t1);
-  f2_unpack(p2, p0, p1);
-  e0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-  e1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
-// max of three that is NaN if one of them is.
-__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 
 // Asks for the work of a block that has not been launched yet; the answer, 16
 // bytes at `answer`, completes `bar`.
@@ -229,8 +199,8 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
   uint64_t* q_full = v_fixed + STAGES;
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;      // [2] S of the tile is in TMEM
-  uint64_t* p_ready = s_full + 2;      // [2] P of 96 keys is in TMEM and O is rescaled
-  uint64_t* p_rest = p_ready + 2;      // [2] P of the other 32
+  uint64_t* p_ready = s_full + 2;      // [2] P of the first keys is in TMEM and O is rescaled
+  uint64_t* p_rest = p_ready + 2;      // [2] P of the others
   uint64_t* o_full = p_rest + 2;       // [2] the item's last P.V is added to O
   uint64_t* work_full = o_full + 2;    // [2]
   uint64_t* work_empty = work_full + 2;  // [2]
@@ -417,11 +387,11 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
               ok = wait(&p_ready[x], (done >> x) & 1);
               if (!ok) break;
               tc_fence_after();
-              issue_pv<T, DP, 0, 6>(o_tmem, s_tmem, vd, j != 0);
+              issue_pv<T, DP, 0, 2 * kEarly>(o_tmem, s_tmem, vd, j != 0);
               ok = wait(&p_rest[x], (done >> x) & 1);
               if (!ok) break;
               tc_fence_after();
-              issue_pv<T, DP, 6, 8>(o_tmem, s_tmem, vd, 1);
+              issue_pv<T, DP, 2 * kEarly, 8>(o_tmem, s_tmem, vd, 1);
               done ^= 1u << x;
               if (x == last) tc_commit_warp(&empty[sv]);
               if (!more) tc_commit_warp(&o_full[x]);
@@ -592,17 +562,14 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int k = 0; k < 64; ++k)
-          mx4[k & 3] = fmax3_nan(mx4[k & 3], __uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1]));
-        const float mx = fmax3_nan(fmax3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], mx4[3]) * p.scale_log2;
+          mx4[k & 3] = fmax3(mx4[k & 3], __uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1]));
+        const float mx = fmaxf(fmax3(mx4[0], mx4[1], mx4[2]), mx4[3]) * p.scale_log2;
         float alpha = 1.f;
         if (mx > m + kStaleMax || (m == -INFINITY && mx > -INFINITY)) {
           alpha = part_weight(m, mx);
           l *= alpha;
           m = mx;
         }
-        // A NaN or +inf score makes its row NaN, as inf - inf does; it goes
-        // into the sum here, since exp2_pair would lose it.
-        if (!(mx < INFINITY)) l = NAN;
         if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
           // (P.V of the tile before this one precedes S in the tensor pipe)
 #pragma unroll
@@ -627,18 +594,14 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
             const uint64_t x2 =
                 f2_fma(f2_pack(__uint_as_float(sv[at]), __uint_as_float(sv[at + 1])), sc2, ng2);
             float e0, e1;
-            if ((k & 3) == 3) {
-              exp2_pair(x2, e0, e1);
-            } else {
-              f2_unpack(x2, e0, e1);
-              e0 = fast_exp2(e0);
-              e1 = fast_exp2(e1);
-            }
+            f2_unpack(x2, e0, e1);
+            e0 = fast_exp2(e0);
+            e1 = fast_exp2(e1);
             sum2[k & 1] = f2_add(sum2[k & 1], f2_pack(e0, e1));
             pk[k] = pack2<T>(e0, e1);
           }
           tmem_st16(s_tmem + c * 16, pk);
-          if (c == 2) {  // P.V may start on three quarters of the keys
+          if (c == kEarly - 1) {  // P.V may start on the keys so far
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(&p_ready[x]);
