@@ -97,8 +97,11 @@ struct Plan {
 };
 
 // Rows (new tokens x heads of a group) up to which the rows kernel takes a
-// sequence when all are that short: its four 16-row warps.
-constexpr int kRowsMost = 64;
+// sequence when all are that short. With 128-wide heads the tile kernel is the
+// faster one from 33 rows on (24 sequences of 8000 keys, 4 key heads, 48 rows:
+// 113 against 127 us; 2 of 60000: 65 against 95), with 64-wide ones it is not
+// (107 against 94 us at 8000 keys).
+constexpr int kRowsMost = 64, kRowsMostWide = 32;
 constexpr int kRowsMinUnits = 2, kTilesMinUnits = 4;
 
 size_t up256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
@@ -112,7 +115,7 @@ Plan make_plan(const pkb200_paged_cache* c, const pkb200_paged_batch* b, int q_h
   const long long most = max_q_len < T ? max_q_len : T;
   const long long rows = most * G;  // of the longest sequence
   const bool tiles_can = pl.dp <= 128 && G <= 128;
-  if (rows <= kRowsMost || !tiles_can) {
+  if (rows <= (pl.dp == 128 ? kRowsMostWide : kRowsMost) || !tiles_can) {
     pl.rows_mr = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     pl.rows_max = 0x7fffffff;
   } else {
