@@ -142,8 +142,11 @@ Plan make_plan(const pkb200_paged_cache* c, const pkb200_paged_batch* b, int q_h
     pl.rows_meta = take(static_cast<size_t>(pl.rows_grid) * sizeof(paged::Entry));
   }
   if (pl.tiles) {
-    const long long per = 2 * (128 / G);  // tokens of a block
-    const long long n = (T + B * (per - 1)) / per;
+    // Row tiles: every sequence of the tile kernel may end in one that is not full,
+    // and has more rows than the rows kernel takes.
+    const long long per = 2 * (128 / G);  // tokens of a row tile
+    const long long least = pl.rows_mr ? pl.rows_max / G + 1 : 1, seqs = B < T / least ? B : T / least;
+    const long long n = (T + seqs * (per - 1)) / per;
     const long long blocks = n * c->heads;
     // Split the keys where that fills the SMs better: time in key tiles of the
     // last block to finish, with 8 tiles' worth for a block's start and end.

@@ -64,6 +64,11 @@ void check_in_place(const Tensor& out, const char* name, const Tensor& in) {
   if (out.data_ptr() == in.data_ptr() && out.strides() != in.strides())
     bad_value(name, " may be the input itself, not another view of its memory");
 }
+// Memory that is written must not be one place under several indexes.
+void check_written(const Tensor& t, const char* name) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) == 0) bad_value(name, " must not be an expanded tensor");
+}
 // 16-byte rows: what the copies of attention start on.
 void check_aligned(const Tensor& t, const char* name) {
   bool ok = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
@@ -119,6 +124,7 @@ Tensor rope(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, bo
     y = *out;
     check_rows(y, "out", x.scalar_type(), dev, x.sizes());
     check_in_place(y, "out", x);
+    check_written(y, "out");
   } else {
     y = at::empty(x.sizes(), x.options());
   }
@@ -207,6 +213,8 @@ py::object paged_kv_append(const Tensor& k, const Tensor& v, const Tensor& k_pag
   const Paged p = paged(k_pages, v_pages, page_table, cu_seqlens, seq_lens, n);
   const at::ScalarType type = k_pages.scalar_type();
   const int64_t heads = p.cache.heads, dim = p.cache.dim;
+  check_written(k_pages, "k_pages");
+  check_written(v_pages, "v_pages");
   check_rows(k, "k", type, p.device, {n, heads, dim});
   check_rows(v, "v", type, p.device, {n, heads, dim});
   if (!inv_freq && (q || q_out)) bad_value("q is only rotated: it needs inv_freq");
@@ -225,6 +233,7 @@ py::object paged_kv_append(const Tensor& k, const Tensor& v, const Tensor& k_pag
       rotated = *q_out;
       check_rows(rotated, "q_out", type, p.device, q->sizes());
       check_in_place(rotated, "q_out", *q);
+      check_written(rotated, "q_out");
     } else {
       rotated = at::empty(q->sizes(), q->options());
     }
@@ -269,6 +278,7 @@ py::object paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor&
     out = *out_arg;
     check_rows(out, "out", q.scalar_type(), p.device, q.sizes());
     check_aligned(out, "out");
+    check_written(out, "out");
   } else {
     out = at::empty(q.sizes(), q.options());
   }

@@ -421,40 +421,57 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
       // ------------------------------------------------------------- work --
       // Items in block order: row tiles fastest, a sequence's longest first,
       // then key heads, then pieces of the keys, so that items which run
-      // together share keys in L2.
+      // together share keys in L2. The grid is the host's bound on them; the
+      // blocks past the batch's own row tiles have nothing to do.
+      // Lane i counts the row tiles of the i-th run of sequences.
+      const int each = (p.B + 31) / 32, b0 = min(p.B, lane * each), b1 = min(p.B, b0 + each);
+      auto tiles_of = [&](const Seq& s) {
+        const int rows = s.nq * p.G;
+        return rows >= p.min_rows && rows <= p.max_rows ? (s.nq + 2 * tok - 1) / (2 * tok) : 0;
+      };
+      int mine = 0;
+#pragma unroll 4
+      for (int b = b0; b < b1; ++b) mine += tiles_of(load_seq(p, b, true));
+      int upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      // (the host's bound holds for sequences that do not overlap; where offsets
+      // run backwards and they do, what is above it is left out)
+      const int total = min(__shfl_sync(0xffffffffu, upto, 31), p.tiles);
+      const int rows_all = total * p.Hkv;  // row tiles of all heads
       int block = blockIdx.x;
-      bool report = true;
       int asked = 0;
       for (;; ++asked) {
-        const int tile = block % p.tiles, hk = block / p.tiles % p.Hkv, split = block / p.tiles / p.Hkv;
-        const int entry = hk * p.tiles + tile;
-        // the sequence that has this row tile, 32 sequences at a time
         TileWork w;
         w.b = -1;
         Seq s;
-        int n_of = 0, before = 0;
-        for (int b0 = 0; b0 < p.B; b0 += 32) {
-          int n = 0;
-          if (b0 + lane < p.B) {
-            s = load_seq(p, b0 + lane, report);
-            const int rows = s.nq * p.G;
-            n = rows >= p.min_rows && rows <= p.max_rows ? (s.nq + 2 * tok - 1) / (2 * tok) : 0;
+        int split = 0, entry = 0, tile = 0, hk = 0, n_of = 0, before = 0;
+        if (block < rows_all * p.splits) {
+          split = block / rows_all;
+          entry = block - split * rows_all;
+          hk = entry / total;
+          tile = entry - hk * total;
+          // the lane whose sequences have this row tile, and the sequence
+          const int from = __ffs(__ballot_sync(0xffffffffu, upto > tile)) - 1;
+          int b = b0, first = upto - mine, n = 0;
+          if (lane == from) {
+            while (true) {
+              n = tiles_of(load_seq(p, b));
+              if (tile < first + n) break;
+              first += n;
+              ++b;
+            }
           }
-          int upto = n;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
-          }
-          const uint32_t hit = __ballot_sync(0xffffffffu, before + upto > tile);
-          if (hit) {
-            const int from = __ffs(hit) - 1;
-            w.b = b0 + from;
-            n_of = __shfl_sync(0xffffffffu, n, from);
-            before = __shfl_sync(0xffffffffu, before + upto - n, from);
-            break;
-          }
-          before += __shfl_sync(0xffffffffu, upto, 31);
+          w.b = __shfl_sync(0xffffffffu, b, from);
+          n_of = __shfl_sync(0xffffffffu, n, from);
+          before = __shfl_sync(0xffffffffu, first, from);
+        } else if (block - rows_all * p.splits < p.tiles * p.Hkv - rows_all) {
+          entry = rows_all + block - rows_all * p.splits;  // an entry that stays empty
+        } else {
+          split = 1;
         }
         bool live = w.b >= 0;
         w.pieces = 0;
@@ -498,7 +515,6 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
           __syncwarp();
           ++item;
         }
-        report = false;
         // The next block is asked for when this item's loads are nearly done and
         // not before: what a block holds back, an idle one cannot take.
         if (live && !wait(ask, (item - 1) & 1)) break;

@@ -457,3 +457,84 @@ def test_wrong_batches(ops, case):
         wrong[3] = bad
         out = ops.paged_attention(q, kp, vp, table, wrong, lens, max_q_len=most)
         assert device_error() == 8 and others(out, 2)
+
+
+@pytest.mark.parametrize("case", [([1, 3], [9, 300], 16, 2, 4, 8), ([200, 1], [200, 77], 16, 1, 4, 8),
+                                  ([90], [700], 16, 1, 2, 40)], ids=str)
+def test_narrow_heads_and_sliced_table(ops, case):
+    q, kp, vp, table, cu, lens = make(*case, torch.bfloat16)
+    wide = torch.full((table.shape[0], table.shape[1] + 5), -7, dtype=torch.int32, device="cuda")
+    wide[:, 2:-3] = table
+    check(ops, (q, kp, vp, wide[:, 2:-3], cu, lens), max_q_len=max(case[0]))
+
+
+@pytest.mark.parametrize("max_q_len", [None, 1, 300])
+def test_many_sequences(ops, max_q_len):
+    """Single tokens, drafts and prompts in one batch of several hundred."""
+    B = 300
+    new = [1 if b % 7 else (300 if b == 140 else 1 + b % 40) for b in range(B)]
+    new[3] = new[200] = 0
+    total = [n + (b * 37) % 200 for b, n in enumerate(new)]
+    check(ops, make(new, total, 16, 1, 4, 64, torch.bfloat16), max_q_len=max_q_len)
+
+
+def test_overlapping_sequences_are_safe(ops):
+    """Offsets that run backwards make sequences overlap, more rows than the tensors
+    have: nothing is written out of range, and the error is reported."""
+    new, total, page = [400, 30, 400], [400, 30, 400], 16
+    q, kp, vp, table, cu, lens = make(new, total, page, 2, 2, 128, torch.bfloat16, pad=0)
+    n = q.shape[0]
+    cu.copy_(torch.tensor([0, n, 0, n], dtype=torch.int32))
+    lens.fill_(int(table.shape[1]) * page)
+    table.clamp_(min=0)
+    room = torch.full((n + 64, *q.shape[1:]), 7.0, device="cuda", dtype=q.dtype)
+    ops.paged_attention(q, kp, vp, table, cu, lens, max_q_len=n, out=room[32:32 + n])
+    assert device_error() == 8
+    assert bool((room[:32] == 7).all()) and bool((room[32 + n:] == 7).all())
+
+
+def test_expanded_outputs_are_refused(ops):
+    q, kp, vp, table, cu, lens = make([2, 1], [20, 9], 16, 2, 2, 64, torch.bfloat16)
+    f = torch.ones(8, device="cuda")
+    pos = torch.zeros(q.shape[0], dtype=torch.int64, device="cuda")
+    same = torch.zeros_like(q[:, :1]).expand_as(q)
+    with pytest.raises(ValueError):
+        ops.rope(q, pos, f, out=same)
+    with pytest.raises(ValueError):
+        ops.paged_attention(q, kp, vp, table, cu, lens, out=same)
+    with pytest.raises(ValueError):
+        ops.paged_kv_append(q[:, :2], q[:, :2], kp[:1].expand_as(kp), vp, table, cu, lens)
+    # expanded inputs are fine
+    one = q[:, :1].expand_as(q)
+    assert torch.equal(ops.rope(one, pos + 3, f), ops.rope(one.contiguous(), pos + 3, f))
+    n, used = int(cu[-1]), table[0, :1].long()
+    shared = kp[used].nan_to_num(0.5).expand_as(kp)  # one page under every index
+    for most in (2, 100):
+        got = ops.paged_attention(one, shared, vp, table, cu, lens, max_q_len=most)[:n]
+        want = ops.paged_attention(one.contiguous(), shared.contiguous(), vp, table, cu, lens, max_q_len=most)[:n]
+        assert torch.equal(got, want)
+
+
+def test_two_threads_at_once(ops):
+    """Calls from several host threads, each on a stream of its own."""
+    import threading
+    cases = [ROWS[3], TILES[4], ROWS[4], TILES[3]]
+    made = [make(*c, torch.bfloat16, seed=i) for i, c in enumerate(cases)]
+    want = [ops.paged_attention(*a, max_q_len=max(c[0]))[:sum(c[0])].clone() for a, c in zip(made, cases)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = ops.paged_attention(*made[i], max_q_len=max(cases[i][0]))[:sum(cases[i][0])]
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(got, want[i]):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
