@@ -19,6 +19,13 @@
 // the second product costs nothing that the reads do not hide. With 64 rows the
 // tensor work (8 cycles per mma.sync and sub-partition) comes near the time of the
 // reads, and P is rounded once to the inputs' type, as in the tile kernel.
+//
+// Measured (8 key heads of 128, groups of 4, bf16): 64 sequences of up to 16k
+// keys, 2.2 GB, in 388 to 403 us: 5.5 to 5.7 TB/s, where a kernel that only reads
+// reaches 5.2. One token over 4096 keys takes 12.3 us, of which the reads are 2.6:
+// two launches, the cut of the line, one tile's latency and the join. With 48
+// rows of 64-wide heads the chain of a tile (S, softmax, P.V: 3100 cycles in one
+// warp, two to a sub-partition) bounds it: 53 us against 15 for the reads.
 #pragma once
 
 #include "paged_common.cuh"

@@ -30,6 +30,14 @@
 // are independent, so the output's stays at the level of its own rounding.
 // The row sums are of the unrounded P, in fp32.
 //
+// Measured (bf16, 128-wide heads): an 8190-token prompt of 32 heads on 8 key heads
+// 530 us, 1037 TFLOP/s (0.64 of the burst matrix rate, 0.76 of the sustained one;
+// the run is power capped at 1.7 GHz); 4 x 32 heads x 2048 tokens over 4096 keys 450
+// us, 917 TFLOP/s; 509 tokens of 28 heads on 4 over 130k keys 959 us, 991 TFLOP/s. A
+// key tile takes a pair of row tiles 3400 cycles: their chains (S, softmax, P.V,
+// and the hand-overs between) alternate, and the tensor pipe waits a third of
+// the time; an item's begin and end cost 5000 to 9000 cycles more.
+//
 // With few row tiles over a long cache, `splits` items share a tile's keys and
 // paged_join_kernel adds their pieces up.
 #pragma once
