@@ -115,14 +115,16 @@ Plan make_plan(const pkb200_paged_cache* c, const pkb200_paged_batch* b, int q_h
   const long long most = max_q_len < T ? max_q_len : T;
   const long long rows = most * G;  // of the longest sequence
   const bool tiles_can = pl.dp <= 128 && G <= 128;
-  if (rows <= (pl.dp == 128 ? kRowsMostWide : kRowsMost) || !tiles_can) {
+  const int few = pl.dp == 128 ? kRowsMostWide : kRowsMost;
+  if (rows <= few || !tiles_can) {
     pl.rows_mr = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
     pl.rows_max = 0x7fffffff;
   } else {
     pl.tiles = true;
     // Single tokens among the prompts go to the rows kernel, unless the sizes
-    // say that there are none.
-    if (B > 1 && T < B * most && G <= kRowsMost) {
+    // say that there are none. (With G <= few the longest sequence has more rows
+    // than rows_max, so that the tile kernel's bound on row tiles is at least one.)
+    if (B > 1 && T < B * most && G <= few) {
       pl.rows_mr = G <= 16 ? 16 : G <= 32 ? 32 : 64;
       pl.rows_max = pl.rows_mr;
     }

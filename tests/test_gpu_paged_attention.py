@@ -493,6 +493,15 @@ def test_overlapping_sequences_are_safe(ops):
     assert bool((room[:32] == 7).all()) and bool((room[32 + n:] == 7).all())
 
 
+@pytest.mark.parametrize("max_q_len", [None, 1, 2])
+@pytest.mark.parametrize("new, group, dim", [([0, 1], 40, 128), ([1, 0, 0, 1], 64, 128), ([0, 1], 33, 72),
+                                             ([0, 2], 33, 128), ([0, 1], 70, 64), ([0, 1, 0], 128, 128)], ids=str)
+def test_fewer_tokens_than_sequences_and_wide_groups(ops, new, group, dim, max_q_len):
+    """Single tokens whose group alone is too many rows for the kernel of few rows."""
+    total = [40 + 300 * i for i in range(len(new))]
+    check(ops, make(new, total, 16, 1, group, dim, torch.bfloat16, pad=0), max_q_len=max_q_len)
+
+
 def test_expanded_outputs_are_refused(ops):
     q, kp, vp, table, cu, lens = make([2, 1], [20, 9], 16, 2, 2, 64, torch.bfloat16)
     f = torch.ones(8, device="cuda")
