@@ -290,7 +290,7 @@ py::object paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor&
   } else if (return_lse) {
     lse = at::empty({n, hq}, q.options().dtype(at::kFloat));
   }
-  const int win = window ? static_cast<int>(std::min<int64_t>(*window, 1 << 30)) : 0;
+  const int win = window ? static_cast<int>(std::min<int64_t>(*window, 0x7fffffff)) : 0;
   const int64_t need = static_cast<int64_t>(pkb200_paged_attention_workspace_size(
       &p.cache, &p.batch, static_cast<int>(hq), static_cast<int>(most), win));
   Tensor ws;

@@ -40,7 +40,7 @@ PKB_INDEX int clip_hi(const Seq& s, int i, int causal) {
   return causal ? least(s.len, s.pos0 + i + 1) : s.len;
 }
 PKB_INDEX int clip_lo(const Seq& s, int i, int window) {
-  return window ? most(0, s.pos0 + i - window + 1) : 0;
+  return window && s.pos0 + i >= window ? s.pos0 + i - window + 1 : 0;  // (no step leaves 32 bits)
 }
 
 // Key tiles of `kt` keys that the tokens [first, last] need, from tile0 on: at

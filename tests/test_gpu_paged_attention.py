@@ -307,6 +307,26 @@ def test_far_pages(ops):
         check(ops, (q, kp, vp, table, cu, lens), max_q_len=max_q_len)
 
 
+def test_window_past_two_to_the_30(ops):
+    """A window of more than 2^30 keys is kept exactly: its first key, among 2^30 + 1024
+    of one shared page, is the one that decides the output."""
+    page, n, window = 1024, 2 ** 30 + 1024, 2 ** 30 + 5
+    kp = torch.zeros(2, 1, page, 8, device="cuda", dtype=torch.bfloat16)
+    vp = torch.zeros_like(kp)
+    table = torch.zeros(1, n // page, dtype=torch.int32, device="cuda")
+    first = n - window
+    table[0, first // page] = 1
+    kp[1, 0, first % page] = 8.0  # a score of 8 * 8 = 64 natural units above all others
+    vp[1, 0, first % page] = 3.0
+    q = torch.ones(1, 1, 8, device="cuda", dtype=torch.bfloat16)
+    cu = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    # the others' weight, 2^30.1 exp(-64), is below a half step of 3 by far
+    got = ops.paged_attention(q, kp, vp, table, cu, lens, window=window, scale=1.0)
+    assert bool((got == 3.0).all())
+    assert bool((ops.paged_attention(q, kp, vp, table, cu, lens, window=window - 1, scale=1.0) == 0.0).all())
+
+
 def test_prompt_then_tokens(ops):
     """The operators as a program uses them: a projection, its split, the rotated
     append and attention, for a ragged prompt and then token by token, against
