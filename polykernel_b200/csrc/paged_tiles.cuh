@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
       // in turn: with a warp for each, their MMAs interleave in the tensor pipe,
       // both softmaxes wait at once, and the pipe runs dry. The loop is kept
       // short (one place for S, one for P.V): all roles share the instruction
-      // cache with the softmax, whose unrolled loop alone is some 25 KB.
+      // cache with the softmax, whose loop is unrolled over a whole tile of keys.
       const uint64_t q_desc = make_sw128_desc(smem_u32(smem), 16, 1024);
       const uint64_t k_desc = make_sw128_desc(smem_u32(smem + C::OFF_KV), 16, 1024);
       const uint64_t v_desc = make_sw128_desc(smem_u32(smem + C::OFF_KV), KT * 128, 1024);
@@ -439,16 +439,18 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
       };
       int mine = 0;
 #pragma unroll 4
-      for (int b = b0; b < b1; ++b) mine += tiles_of(load_seq(p, b, true));
+      for (int b = b0; b < b1; ++b) mine = min(mine + tiles_of(load_seq(p, b, true)), p.tiles);
+      // (the host's bound holds for sequences that do not overlap; where offsets
+      // run backwards and they do, what is above it is left out)
       int upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += y;
+        if (lane >= o) upto = min(upto + y, p.tiles);
       }
-      // (the host's bound holds for sequences that do not overlap; where offsets
-      // run backwards and they do, what is above it is left out)
-      const int total = min(__shfl_sync(0xffffffffu, upto, 31), p.tiles);
+      const int total = __shfl_sync(0xffffffffu, upto, 31);
+      int ahead = __shfl_up_sync(0xffffffffu, upto, 1);  // row tiles of the lanes before
+      if (lane == 0) ahead = 0;
       const int rows_all = total * p.Hkv;  // row tiles of all heads
       int block = blockIdx.x;
       int asked = 0;
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
           tile = entry - hk * total;
           // the lane whose sequences have this row tile, and the sequence
           const int from = __ffs(__ballot_sync(0xffffffffu, upto > tile)) - 1;
-          int b = b0, first = upto - mine, n = 0;
+          int b = b0, first = ahead, n = 0;
           if (lane == from) {
             while (true) {
               n = tiles_of(load_seq(p, b));
