@@ -390,6 +390,13 @@ int pkb200_last_gemm_config(int* cfg7);
  * timeout); the CUDA context stays usable. New; no reference counterpart. */
 int pkb200_selftest_wait_timeout(long long limit_cycles, int* code);
 
+/* Failure-detection self test of pkb200_paged_attention for few rows per key
+ * head: later calls wait for at most wait_limit SM clocks for a tile, and begin
+ * to fetch after hold_back clocks (both at most ~2 s). With hold_back above
+ * wait_limit their blocks give up: the call ends, its output is undefined and
+ * the error word is 4. (0, 0) restores the defaults. Process-wide. */
+int pkb200_selftest_paged_limits(long long wait_limit, long long hold_back);
+
 /* ---- serving engine ABI. The reference's Modal app binds
  *   int polykernel_fused_mlp_block(float* in, float* out, int M, int N, int K)
  * through ctypes (modal/app.py:206-215, 795, 836) but no library in the

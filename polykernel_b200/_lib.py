@@ -70,6 +70,7 @@ SIGNATURES = {
     "pkb200_paged_attention_workspace_size": (c_size_t, [_P, _P, c_int, c_int, c_int]),
     "pkb200_paged_attention": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int,
                                        c_float, _P, c_size_t, _P]),
+    "pkb200_selftest_paged_limits": (c_int, [c_longlong, c_longlong]),
     "pkb200_set_gemm_max_ctas": (c_int, [c_int]),
     "pkb200_device_arch": (c_int, [ctypes.c_char_p, c_size_t]),
     "pkb200_tuning_load": (c_int, [ctypes.c_char_p, ctypes.c_char_p, c_size_t]),

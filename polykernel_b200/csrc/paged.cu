@@ -1,6 +1,7 @@
 // paged.cu - C ABI of the paged-cache operators (include/pkb200.h): rotary
 // positions, the append of new keys and values, and attention over the cache.
 // Host-side checks, launch shapes and the choice between kernels.
+#include <atomic>
 #include <cmath>
 
 #include "internal.h"
@@ -12,6 +13,9 @@
 using namespace pkb200;
 
 namespace {
+
+// pkb200_selftest_paged_limits
+std::atomic<long long> g_wait_limit{kSpinLimitCycles}, g_hold_back{0};
 
 cudaStream_t S(void* s) { return static_cast<cudaStream_t>(s); }
 
@@ -488,9 +492,19 @@ int pkb200_paged_attention(const pkb200_paged_cache* cache, const pkb200_paged_b
   a.window = window;
   a.scale_log2 = scale * 1.4426950408889634f;  // log2(e)
   a.err = err;
+  a.wait_limit = g_wait_limit.load(std::memory_order_relaxed);
+  a.hold_back = g_hold_back.load(std::memory_order_relaxed);
   char* ws = static_cast<char*>(workspace);
   return cache->dtype == PKB200_BF16 ? launch_attention<__nv_bfloat16>(cache, a, pl, ws, S(stream))
                                      : launch_attention<__half>(cache, a, pl, ws, S(stream));
+}
+
+int pkb200_selftest_paged_limits(long long wait_limit, long long hold_back) {
+  if (wait_limit < 0 || wait_limit > kSpinLimitCycles || hold_back < 0 || hold_back > kSpinLimitCycles)
+    return cudaErrorInvalidValue;
+  g_wait_limit = wait_limit ? wait_limit : kSpinLimitCycles;
+  g_hold_back = hold_back;
+  return cudaSuccess;
 }
 
 }  // extern "C"

@@ -45,6 +45,8 @@ struct AttnParams {
   float2* part_ml;     // [slot][rows] their maxima and sums
   int* meta;           // [entry][8], see Entry
   int* err;
+  long long wait_limit;  // rows kernel: cycles after which a wait gives the block up
+  long long hold_back;   // and cycles before its first copies (a self test's, else 0)
 };
 
 // A tile of rows whose pieces the joining pass adds up.

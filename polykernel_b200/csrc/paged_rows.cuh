@@ -79,6 +79,19 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4])
                : "r"(addr));
 }
 __device__ __forceinline__ void compute_warps_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// The same, and whether `ok` holds in all of them: one answer for all four warps.
+__device__ __forceinline__ bool compute_warps_all(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, 1, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"(static_cast<uint32_t>(ok))
+      : "memory");
+  return all != 0;
+}
 
 constexpr int kAhead = 3;  // steps between the load of a fragment and its products
 
@@ -221,6 +234,10 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
     int slot = 0, issued = 0;
     uint32_t parity = 1;
     bool ok = true;
+    if (p.hold_back) {
+      const long long t0 = clock64();
+      while (clock64() - t0 < p.hold_back) {}
+    }
     for (long long u = u0; u < u1 && ok;) {
       const int run = static_cast<int>(min(static_cast<long long>(at.n - off), u1 - u));
       auto lookup = [&](int tile) {  // this lane's page in that key tile
@@ -236,7 +253,7 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
 #pragma unroll
         for (int kv = 0; kv < 2 && ok; ++kv) {
           ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], parity, p.err, abort_flag,
-                                                 kErrTimeoutProducer));
+                                                 kErrTimeoutProducer, p.wait_limit));
           if (!ok) break;
           if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
           __syncwarp();
@@ -315,7 +332,8 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
       float s[KW / 8][4];
 #pragma unroll
       for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-      ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], parity, p.err, abort_flag, kErrTimeoutSoftmax));
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], parity, p.err, abort_flag, kErrTimeoutSoftmax,
+                                               p.wait_limit));
       if (!ok) break;
       {
         const uint32_t base = slots_addr + slot * C::SLOT;
@@ -406,7 +424,8 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
         l_b = x + y;
       }
       // ---- O += P V
-      ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], parity, p.err, abort_flag, kErrTimeoutSoftmax));
+      ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], parity, p.err, abort_flag, kErrTimeoutSoftmax,
+                                               p.wait_limit));
       if (!ok) break;
       const uint32_t base = slots_addr + slot * C::SLOT;
       bool by_hand = false;
@@ -498,7 +517,6 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
         parity ^= 1;
       }
     }
-    if (!ok) break;
 
     // ---- join the warps that took the same rows' keys, through shared memory;
     // rows leave as whole lines: the output, or a piece for the joining pass
@@ -519,7 +537,10 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
         ml_s[warp * 16 + g + 8] = make_float2(m_b, l_b);
       }
     }
-    compute_warps_sync();
+    // A warp whose wait ended without its tile comes here too, and the four leave
+    // together: a barrier that one of them never reaches would hold the others for good.
+    ok = compute_warps_all(ok);
+    if (!ok) break;
     const bool begins = off == 0, ends = off + run == at.n;
     const bool whole = begins && ends;
     const long long slot_row = (2LL * blockIdx.x + (begins ? 1 : 0)) * MR;
