@@ -444,6 +444,7 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
           }
         }
         fence_proxy_async_smem();
+        __syncwarp();  // other lanes read what was cleared here, and a vote orders no memory
         by_hand = __any_sync(0xffffffffu, bad);
       }
       if (!by_hand) {
