@@ -108,6 +108,141 @@ __device__ __forceinline__ uint32_t not_finite4(const uint4& w) {
   return t & 0x80008000u;
 }
 
+// The same values with zeros in the place of those.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_only(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  return w & ~__vcmpeq2(w & e, e);
+}
+template <typename T>
+__device__ __forceinline__ uint4 finite_only4(const uint4& w) {
+  return make_uint4(finite_only<T>(w.x), finite_only<T>(w.y), finite_only<T>(w.z), finite_only<T>(w.w));
+}
+
+// mbar_wait for a role whose wait may last as long as others go over many keys
+// again (mark_values): the limit runs anew while they count `alive` up.
+__device__ __forceinline__ bool mbar_wait_alive(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag,
+                                                int code, long long limit, const volatile int* alive) {
+  if (mbar_try_wait(bar, parity)) return true;
+  long long t0 = clock64();
+  int seen = *alive;
+  while (true) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (clock64() - t0 > limit) {
+      const int now = *alive;
+      if (now == seen) {
+        atomicCAS(err, 0, code);
+        *abort_flag = 1;
+        return false;
+      }
+      seen = now;
+      t0 = clock64();
+    }
+  }
+}
+
+// --------------------------------------------- values that are not finite --
+// A visible key's weight is positive, so a value of it that is infinite decides
+// its column: inf of its sign, or NaN with one of the other sign, or if a value is
+// NaN. Products formed from weights of 16 bits do not keep that: a weight may round
+// to 0, or be split into a value and a remainder of the other sign, and 0 * inf and
+// inf - inf are NaN. So where a finished row is not finite although its sum of
+// exponentials is, or where values were taken out of a tile (finite_only), the kernels
+// go over the values of its keys again (rare, and as fast as they can be read)
+// and mark what decides its columns.
+//
+// A row's marks are 2 W words, W = DP / 32: column d is bit d / W of word d % W; the first
+// W words are for inf, the others for -inf, NaN is both. (Lane i reads columns W i ... W i + W - 1.)
+template <typename T, int DP>
+__device__ __forceinline__ void load_values(const void* row, bool mine, uint32_t (&w)[DP / 64]) {
+  const uint32_t* src = static_cast<const uint32_t*>(row) + lane_id() * (DP / 64);
+#pragma unroll
+  for (int c = 0; c < DP / 64; ++c) w[c] = mine ? __ldg(src + c) : 0u;
+}
+template <typename T, int N>
+__device__ __forceinline__ bool any_not_finite(const uint32_t (&w)[N]) {
+  bool bad = false;
+#pragma unroll
+  for (int c = 0; c < N; ++c) bad |= finite_only<T>(w[c]) != w[c];
+  return bad;
+}
+
+// One warp, for `rows` rows of a sequence from row0 on (at most 32), one per lane, and those
+// of the keys [k0, k1) that they see. One lane calls `alive` on the way, for those who wait.
+template <typename T, int DP, class Alive>
+__device__ __forceinline__ void mark_values(const AttnParams& p, int b, int hk, const Seq& s, int row0, int rows,
+                                            int k0, int k1, uint32_t (&marks)[DP / 16], Alive alive) {
+  constexpr int W = DP / 32, N = DP / 64;
+  const int lane = lane_id();
+#pragma unroll
+  for (int c = 0; c < 2 * W; ++c) marks[c] = 0u;
+  if (rows <= 0) return;
+  const int token = (row0 + min(lane, rows - 1)) / p.G;
+  const int lo = key_lo(p, s, token), hi = key_hi(p, s, token);
+  const int from = max(k0, __shfl_sync(0xffffffffu, lo, 0)), to = min(k1, __shfl_sync(0xffffffffu, hi, 31));
+  const bool mine = lane * W < p.D;
+  auto place = [&](const void* pool, long long sp, long long sh, long long sr, int page, int row) -> const void* {
+    return static_cast<const T*>(pool) + page * sp + hk * sh + row * sr;
+  };
+  for (int j0 = from; j0 < to; j0 += 32) {
+    int page = p.num_pages, row = 0;  // of key j0 + lane; a page outside the pool has zeros
+    if (j0 + lane < to) {
+      page = clip_page(__ldg(p.table + b * p.table_stride + (j0 + lane) / p.page_size), p.num_pages);
+      row = (j0 + lane) % p.page_size;
+    }
+    for (int i0 = 0; i0 < 32 && j0 + i0 < to; i0 += 8) {
+      uint32_t which = 0;  // of the next eight keys
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int pg = __shfl_sync(0xffffffffu, page, i0 + i), r = __shfl_sync(0xffffffffu, row, i0 + i);
+        uint32_t w[N];
+        load_values<T, DP>(place(p.v, p.vp_p, p.vp_h, p.vp_r, pg, r), mine && pg < p.num_pages, w);
+        which |= static_cast<uint32_t>(any_not_finite<T>(w)) << i;
+      }
+      which = __reduce_or_sync(0xffffffffu, which);
+      while (which) {
+        const int i = i0 + __ffs(which) - 1, key = j0 + i;
+        which &= which - 1;
+        const int pg = __shfl_sync(0xffffffffu, page, i), r = __shfl_sync(0xffffffffu, row, i);
+        uint32_t w[N], kw[N], up[W], down[W];
+        load_values<T, DP>(place(p.v, p.vp_p, p.vp_h, p.vp_r, pg, r), mine, w);
+        load_values<T, DP>(place(p.k, p.kp_p, p.kp_h, p.kp_r, pg, r), mine, kw);
+#pragma unroll
+        for (int c = 0; c < W; ++c) {
+          const float2 two = unpack2<T>(w[c / 2]);
+          const float v = c % 2 ? two.y : two.x;
+          up[c] = __ballot_sync(0xffffffffu, v != v || v == INFINITY);
+          down[c] = __ballot_sync(0xffffffffu, v != v || v == -INFINITY);
+        }
+        // A key that is not finite scores inf or NaN, and the row's sum is NaN
+        // whatever is marked, or -inf: its weight is 0 and the product with it NaN.
+        const bool odd_key = __any_sync(0xffffffffu, any_not_finite<T>(kw));
+        if (odd_key) {
+#pragma unroll
+          for (int c = 0; c < W; ++c) up[c] = down[c] = up[c] | down[c];
+        }
+        if (key >= lo && key < hi) {
+#pragma unroll
+          for (int c = 0; c < W; ++c) {
+            marks[c] |= up[c];
+            marks[W + c] |= down[c];
+          }
+        }
+      }
+    }
+    if (lane == 0) alive();
+  }
+}
+
+// Column d of a row with those marks, o where it has none.
+template <int DP>
+__device__ __forceinline__ float marked(float o, const uint32_t (&marks)[DP / 16], int d) {
+  constexpr int W = DP / 32;
+  const bool up = marks[d % W] >> (d / W) & 1u, down = marks[W + d % W] >> (d / W) & 1u;
+  return up ? (down ? NAN : INFINITY) : down ? -INFINITY : o;
+}
+
 constexpr float kStaleMax = 8.f;  // log2 units a row's maximum may lag behind
 
 // Weight of a part whose maximum is m within a row whose maximum is top.
@@ -196,7 +331,34 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttnPara
       add(ml.x, ml.y, ok);
     }
   };
+  // The same for a row with infinities: a weight that is too small for 32 bits is
+  // not 0, and keeps one.
+  auto gather_special = [&](int row) {
+    gather(row, 0, 1);
+    const float top = m;
+#pragma unroll
+    for (int c = 0; c < C; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < e.pieces; ++k) {
+      const long long at = static_cast<long long>(k == 0 ? e.slot0 : e.slot1 + (k - 1) * e.step) * slot_rows + row;
+      const float w = part_weight(p.part_ml[at].x, top);
+      auto part = [&](float& to, float x) { to += w != 0.f ? x * w : fabsf(x) < INFINITY ? 0.f : x; };
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int d = lane * 4 + c * 128;
+        if (d >= DP) continue;
+        const float4 x = *reinterpret_cast<const float4*>(p.part_o + at * DP + d);
+        part(o[c].x, x.x);
+        part(o[c].y, x.y);
+        part(o[c].z, x.z);
+        part(o[c].w, x.w);
+      }
+    }
+  };
   auto store = [&](int row) {
+    bool odd = false;
+#pragma unroll
+    for (int c = 0; c < C; ++c) odd |= !(fabsf(o[c].x) + fabsf(o[c].y) + fabsf(o[c].z) + fabsf(o[c].w) < INFINITY);
+    if (__any_sync(0xffffffffu, odd) && fabsf(l) < INFINITY) gather_special(row);
     const int r = e.row0 + row, tr = r / p.G, h = e.hk * p.G + r - tr * p.G;
     const long long t = e.t0 + tr;
     const float inv = inverse_sum(l);

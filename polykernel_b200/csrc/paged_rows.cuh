@@ -48,8 +48,9 @@ struct RowsCfg {
   static constexpr int STRIDE = DP + 8;
   static constexpr int OFF_STAGE = SLOTS * SLOT;
   static constexpr int OFF_ML = OFF_STAGE + 4 * 16 * STRIDE * 4;  // float2[4][16]
-  static constexpr int OFF_BAR = OFF_ML + 4 * 16 * 8;             // full[SLOTS], empty[SLOTS]
-  static constexpr int OFF_SCAN = OFF_BAR + 2 * SLOTS * 8;        // long long[5], start of the run
+  static constexpr int OFF_MARKS = OFF_ML + 4 * 16 * 8;           // the rows' marks, uint32_t[MR][DP / 16]
+  static constexpr int OFF_BAR = OFF_MARKS + MR * DP / 4;         // full[SLOTS], empty[SLOTS]
+  static constexpr int OFF_SCAN = OFF_BAR + 2 * SLOTS * 8;        // long long[5], start of the run, flags
   static constexpr int SMEM = OFF_SCAN + 5 * 8 + 32 + 1024;
 };
 
@@ -177,6 +178,9 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
   long long* start_rem = scan + 5;
   int* start_b = reinterpret_cast<int*>(scan + 6);
   volatile int* abort_flag = start_b + 1;
+  // [2] values of a run's keys were found that are not finite (by the run's parity)
+  volatile int* special = start_b + 2;
+  volatile int* alive = start_b + 4;  // see mbar_wait_alive
   const int warp = warp_id(), lane = lane_id();
   Entry* const meta = reinterpret_cast<Entry*>(p.meta) + blockIdx.x;
 
@@ -186,7 +190,7 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 4);
     }
-    *abort_flag = 0;
+    *abort_flag = special[0] = special[1] = *alive = 0;
     fence_barrier_init();
   }
   // This block's run [u0, u1) of the batch's key tiles.
@@ -252,8 +256,8 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
         const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, page >= 0)) * p.box * 128;
 #pragma unroll
         for (int kv = 0; kv < 2 && ok; ++kv) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&empty[slot], parity, p.err, abort_flag,
-                                                 kErrTimeoutProducer, p.wait_limit));
+          ok = __all_sync(0xffffffffu, mbar_wait_alive(&empty[slot], parity, p.err, abort_flag,
+                                                       kErrTimeoutProducer, p.wait_limit, alive));
           if (!ok) break;
           if (lane == 0) mbar_arrive_expect_tx(&full[slot], bytes);
           __syncwarp();
@@ -295,6 +299,7 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
   int slot = 0;
   uint32_t parity = 0;
   bool wrote_meta = false;
+  int which = 0;  // parity of the run
   bool ok = true;
 
   for (long long u = u0; u < u1 && ok;) {
@@ -428,26 +433,26 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
                                                p.wait_limit));
       if (!ok) break;
       const uint32_t base = slots_addr + slot * C::SLOT;
-      bool by_hand = false;
       if (masked) {
         // A masked key has P = 0, but 0 * inf and 0 * NaN are NaN. Rows past
-        // the sequence's end (stale memory) are cleared here; values of keys
-        // that only some rows see cannot be, and if one of those is not
-        // finite this tile's products are formed one by one.
+        // the sequence's end (stale memory) are cleared here, and values that are not
+        // finite taken out: the rows that see them get them at the end.
         bool bad = false;
         for (int x = lane; x < KW * HALVES * 8; x += 32) {
           const int key = wk * KW + x / (HALVES * 8), c = x % (HALVES * 8);
           uint4* w = reinterpret_cast<uint4*>(smem + slot * C::SLOT + (c >> 3) * (KT * 128) + key * 128 + (c & 7) * 16);
-          if (key0 + key >= at.s.len) *w = make_uint4(0u, 0u, 0u, 0u);
-          else {
-            bad |= not_finite4<T>(*w) != 0;
+          if (key0 + key >= at.s.len) {
+            *w = make_uint4(0u, 0u, 0u, 0u);
+          } else if (not_finite4<T>(*w)) {
+            *w = finite_only4<T>(*w);
+            bad = true;
           }
         }
+        if (bad) special[which] = 1;
         fence_proxy_async_smem();
-        __syncwarp();  // other lanes read what was cleared here, and a vote orders no memory
-        by_hand = __any_sync(0xffffffffu, bad);
+        __syncwarp();  // other lanes read what was cleared here
       }
-      if (!by_hand) {
+      {
         uint32_t vf[kAhead + 1][4];
         auto load = [&](int i) {
           const int d = i % (DP / 16), key = key_v + i / (DP / 16) * 16, c = (d & 3) * 2 + chunk_v;
@@ -480,36 +485,6 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
             }
           }
         }
-      } else {
-        for (int kk = 0; kk < KW; ++kk) {
-          float pa = 0.f, pb = 0.f;  // this key's P in rows g and g + 8
-#pragma unroll
-          for (int n = 0; n < KW / 8; ++n) {
-            if (n == kk >> 3) {
-              pa = (kk & 1) ? s[n][1] : s[n][0];
-              pb = (kk & 1) ? s[n][3] : s[n][2];
-            }
-          }
-          const int src = (lane & ~3) | ((kk & 7) >> 1);
-          pa = __shfl_sync(0xffffffffu, pa, src);
-          pb = __shfl_sync(0xffffffffu, pb, src);
-          const int k = wk * KW + kk, key = key0 + k;
-          const bool see_a = key >= lo_a && key < hi_a, see_b = key >= lo_b && key < hi_b;
-#pragma unroll
-          for (int d = 0; d < DP / 8; ++d) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(
-                smem + slot * C::SLOT + (d >> 3) * (KT * 128) + k * 128 + (((d & 7) ^ (k & 7)) << 4) + t4 * 4);
-            const float2 v = unpack2<T>(w);
-            if (see_a) {
-              o[d][0] = fmaf(pa, v.x, o[d][0]);
-              o[d][1] = fmaf(pa, v.y, o[d][1]);
-            }
-            if (see_b) {
-              o[d][2] = fmaf(pb, v.x, o[d][2]);
-              o[d][3] = fmaf(pb, v.y, o[d][3]);
-            }
-          }
-        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[slot]);
@@ -528,11 +503,19 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
     }
     {
       float* own = stage + warp * 16 * C::STRIDE;
+      uint64_t na = f2_pack(0.f, 0.f), nb = na;  // 0, NaN once a value is not finite
+      const uint64_t zero = na;
 #pragma unroll
       for (int d = 0; d < DP / 8; ++d) {
+        na = f2_fma(f2_pack(o[d][0], o[d][1]), zero, na);
+        nb = f2_fma(f2_pack(o[d][2], o[d][3]), zero, nb);
         *reinterpret_cast<float2*>(own + g * C::STRIDE + d * 8 + t4 * 2) = make_float2(o[d][0], o[d][1]);
         *reinterpret_cast<float2*>(own + (g + 8) * C::STRIDE + d * 8 + t4 * 2) = make_float2(o[d][2], o[d][3]);
       }
+      float n0, n1, n2, n3;
+      f2_unpack(na, n0, n1);
+      f2_unpack(nb, n2, n3);
+      if ((n0 + n1 != 0.f && fabsf(l_a) < INFINITY) || (n2 + n3 != 0.f && fabsf(l_b) < INFINITY)) special[which] = 1;
       if (t4 == 0) {
         ml_s[warp * 16 + g] = make_float2(m_a, l_a);
         ml_s[warp * 16 + g + 8] = make_float2(m_b, l_b);
@@ -542,6 +525,20 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
     // together: a barrier that one of them never reaches would hold the others for good.
     ok = compute_warps_all(ok);
     if (!ok) break;
+    const bool redo = special[which] != 0;
+    uint4* const marks = reinterpret_cast<uint4*>(smem + C::OFF_MARKS);
+    if (redo) {
+      const int r0 = warp * (MR / 4), rows = min(MR / 4, max(at.rows - at.rt * MR - r0, 0));
+      uint32_t m[DP / 16];
+      mark_values<T, DP>(p, at.b, at.hk, at.s, at.rt * MR + r0, rows, (at.tile0 + off) * KT,
+                         (at.tile0 + off + run) * KT, m, [&] { ++*alive; });
+      if (lane < rows) {
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c)
+          marks[(r0 + lane) * (DP / 64) + c] = make_uint4(m[4 * c], m[4 * c + 1], m[4 * c + 2], m[4 * c + 3]);
+      }
+      compute_warps_sync();
+    }
     const bool begins = off == 0, ends = off + run == at.n;
     const bool whole = begins && ends;
     const long long slot_row = (2LL * blockIdx.x + (begins ? 1 : 0)) * MR;
@@ -568,6 +565,16 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
         v.z = fmaf(x.z, f, v.z);
         v.w = fmaf(x.w, f, v.w);
       }
+      if (redo) {
+        uint32_t m[DP / 16];
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c) {
+          const uint4 w = marks[r * (DP / 64) + c];
+          m[4 * c] = w.x, m[4 * c + 1] = w.y, m[4 * c + 2] = w.z, m[4 * c + 3] = w.w;
+        }
+        v = make_float4(marked<DP>(v.x, m, col), marked<DP>(v.y, m, col + 1), marked<DP>(v.z, m, col + 2),
+                        marked<DP>(v.w, m, col + 3));
+      }
       if (whole) {
         const int tr = seq_row / p.G, h = at.hk * p.G + seq_row - tr * p.G;
         const long long t = at.s.t0 + tr;
@@ -582,6 +589,8 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
       }
     }
     compute_warps_sync();  // the stage is free again
+    if (threadIdx.x == 0) special[which] = 0;  // (the run after next is the first to use it again)
+    which ^= 1;
     if (begins && !ends) {  // only ever the run's last row tile
       wrote_meta = true;
       if (threadIdx.x == 0) {
