@@ -169,68 +169,76 @@ __device__ __forceinline__ bool any_not_finite(const uint32_t (&w)[N]) {
 }
 
 // One warp, for `rows` rows of a sequence from row0 on (at most 32), one per lane, and those
-// of the keys [k0, k1) that they see. One lane calls `alive` on the way, for those who wait.
+// of the keys [k0, k1) that they see; adds to their marks. One lane calls `alive` on the
+// way, for those who wait.
 template <typename T, int DP, class Alive>
 __device__ __forceinline__ void mark_values(const AttnParams& p, int b, int hk, const Seq& s, int row0, int rows,
                                             int k0, int k1, uint32_t (&marks)[DP / 16], Alive alive) {
   constexpr int W = DP / 32, N = DP / 64;
-  const int lane = lane_id();
-#pragma unroll
-  for (int c = 0; c < 2 * W; ++c) marks[c] = 0u;
+  constexpr int ACROSS = DP / 8, KEYS = 32 / ACROSS;  // lanes of a row of 16 bytes each, and rows of a load
   if (rows <= 0) return;
+  const int lane = lane_id();
   const int token = (row0 + min(lane, rows - 1)) / p.G;
   const int lo = key_lo(p, s, token), hi = key_hi(p, s, token);
   const int from = max(k0, __shfl_sync(0xffffffffu, lo, 0)), to = min(k1, __shfl_sync(0xffffffffu, hi, 31));
   const bool mine = lane * W < p.D;
-  auto place = [&](const void* pool, long long sp, long long sh, long long sr, int page, int row) -> const void* {
+  auto place = [&](const void* pool, long long sp, long long sh, long long sr, int page, int row) {
     return static_cast<const T*>(pool) + page * sp + hk * sh + row * sr;
   };
+  auto page_at = [&](int key) {  // a page outside the pool has zeros, keys past the end are none of its
+    return key < to ? clip_page(__ldg(p.table + b * p.table_stride + key / p.page_size), p.num_pages) : p.num_pages;
+  };
+  int page = page_at(from + lane);
   for (int j0 = from; j0 < to; j0 += 32) {
-    int page = p.num_pages, row = 0;  // of key j0 + lane; a page outside the pool has zeros
-    if (j0 + lane < to) {
-      page = clip_page(__ldg(p.table + b * p.table_stride + (j0 + lane) / p.page_size), p.num_pages);
-      row = (j0 + lane) % p.page_size;
-    }
-    for (int i0 = 0; i0 < 32 && j0 + i0 < to; i0 += 8) {
-      uint32_t which = 0;  // of the next eight keys
+    const int row = (j0 + lane) % p.page_size, next = page_at(j0 + 32 + lane);
+    uint32_t which = 0;  // keys with such values
+#pragma unroll
+    for (int i0 = 0; i0 < 32; i0 += 8 * KEYS) {
+      uint4 v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int pg = __shfl_sync(0xffffffffu, page, i0 + i), r = __shfl_sync(0xffffffffu, row, i0 + i);
-        uint32_t w[N];
-        load_values<T, DP>(place(p.v, p.vp_p, p.vp_h, p.vp_r, pg, r), mine && pg < p.num_pages, w);
-        which |= static_cast<uint32_t>(any_not_finite<T>(w)) << i;
+        const int key = (i0 + i * KEYS + lane / ACROSS) & 31;
+        const int pg = __shfl_sync(0xffffffffu, page, key), r = __shfl_sync(0xffffffffu, row, key);
+        const int d = lane % ACROSS * 8;
+        v[i] = pg < p.num_pages && d < p.D
+                   ? __ldg(reinterpret_cast<const uint4*>(place(p.v, p.vp_p, p.vp_h, p.vp_r, pg, r) + d))
+                   : make_uint4(0u, 0u, 0u, 0u);
       }
-      which = __reduce_or_sync(0xffffffffu, which);
-      while (which) {
-        const int i = i0 + __ffs(which) - 1, key = j0 + i;
-        which &= which - 1;
-        const int pg = __shfl_sync(0xffffffffu, page, i), r = __shfl_sync(0xffffffffu, row, i);
-        uint32_t w[N], kw[N], up[W], down[W];
-        load_values<T, DP>(place(p.v, p.vp_p, p.vp_h, p.vp_r, pg, r), mine, w);
-        load_values<T, DP>(place(p.k, p.kp_p, p.kp_h, p.kp_r, pg, r), mine, kw);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (not_finite4<T>(v[i])) which |= 1u << ((i0 + i * KEYS + lane / ACROSS) & 31);
+    }
+    which = __reduce_or_sync(0xffffffffu, which);
+    while (which) {
+      const int i = __ffs(which) - 1, key = j0 + i;
+      which &= which - 1;
+      const int pg = __shfl_sync(0xffffffffu, page, i), r = __shfl_sync(0xffffffffu, row, i);
+      uint32_t w[N], kw[N], up[W], down[W];
+      load_values<T, DP>(place(p.v, p.vp_p, p.vp_h, p.vp_r, pg, r), mine, w);
+      load_values<T, DP>(place(p.k, p.kp_p, p.kp_h, p.kp_r, pg, r), mine, kw);
+#pragma unroll
+      for (int c = 0; c < W; ++c) {
+        const float2 two = unpack2<T>(w[c / 2]);
+        const float v = c % 2 ? two.y : two.x;
+        up[c] = __ballot_sync(0xffffffffu, v != v || v == INFINITY);
+        down[c] = __ballot_sync(0xffffffffu, v != v || v == -INFINITY);
+      }
+      // A key that is not finite scores inf or NaN, and the row's sum is NaN
+      // whatever is marked, or -inf: its weight is 0 and the product with it NaN.
+      const bool odd_key = __any_sync(0xffffffffu, any_not_finite<T>(kw));
+      if (odd_key) {
+#pragma unroll
+        for (int c = 0; c < W; ++c) up[c] = down[c] = up[c] | down[c];
+      }
+      if (key >= lo && key < hi) {
 #pragma unroll
         for (int c = 0; c < W; ++c) {
-          const float2 two = unpack2<T>(w[c / 2]);
-          const float v = c % 2 ? two.y : two.x;
-          up[c] = __ballot_sync(0xffffffffu, v != v || v == INFINITY);
-          down[c] = __ballot_sync(0xffffffffu, v != v || v == -INFINITY);
-        }
-        // A key that is not finite scores inf or NaN, and the row's sum is NaN
-        // whatever is marked, or -inf: its weight is 0 and the product with it NaN.
-        const bool odd_key = __any_sync(0xffffffffu, any_not_finite<T>(kw));
-        if (odd_key) {
-#pragma unroll
-          for (int c = 0; c < W; ++c) up[c] = down[c] = up[c] | down[c];
-        }
-        if (key >= lo && key < hi) {
-#pragma unroll
-          for (int c = 0; c < W; ++c) {
-            marks[c] |= up[c];
-            marks[W + c] |= down[c];
-          }
+          marks[c] |= up[c];
+          marks[W + c] |= down[c];
         }
       }
     }
+    page = next;
     if (lane == 0) alive();
   }
 }

@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
     uint4* const marks = reinterpret_cast<uint4*>(smem + C::OFF_MARKS);
     if (redo) {
       const int r0 = warp * (MR / 4), rows = min(MR / 4, max(at.rows - at.rt * MR - r0, 0));
-      uint32_t m[DP / 16];
+      uint32_t m[DP / 16] = {};
       mark_values<T, DP>(p, at.b, at.hk, at.s, at.rt * MR + r0, rows, (at.tile0 + off) * KT,
                          (at.tile0 + off + run) * KT, m, [&] { ++*alive; });
       if (lane < rows) {

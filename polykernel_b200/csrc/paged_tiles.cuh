@@ -15,8 +15,8 @@
 //                    row's maximum moved by more than 2^8 (P stays below 2^8 and
 //                    the sums share the stale maximum, so the quotient is
 //                    exact), and writes the output.
-//   warps 8-11       clear value rows past the end of a sequence and look for
-//                    values that are not finite in tiles that some row masks.
+//   warps 8-11       clear value rows past the end of a sequence and take values
+//                    that are not finite out of tiles that some row masks.
 //   warp 12          TMA: Q, and key and value pages into one ring.
 //   warp 13          MMA issue, and owner of TMEM.
 //   warp 14          work: blocks stay resident and take over the work of blocks
@@ -75,7 +75,7 @@ struct alignas(64) TileWork {
   int hk, tile0, nt;  // key head, key tiles [tile0, tile0 + nt)
   int pieces, slot;   // pieces of these rows' keys, and where this one goes
   int all_lo, all_hi; // keys that every row sees
-  int by_hand;        // values of masked keys are not finite
+  int special;        // values that are not finite were taken out of masked tiles
 };
 static_assert(sizeof(TileWork) == 64, "");
 
@@ -129,61 +129,47 @@ __device__ __forceinline__ void issue_pv(uint32_t o_tmem, uint32_t p_tmem, uint6
                            kk == FROM ? add : 1u);
 }
 
-// One row's attention over the keys [k0, k1) that it sees, by one warp, in fp32
-// with plain loads: for tiles whose masked values are not finite. Lane d holds
-// outputs d, d + 32, ...
+// Goes over the values of a warp's 32 rows again, and puts what decides their
+// columns into O: all of them if a value in O is not finite (`counts`: of a row for
+// which that matters), else those of masked tiles, from which they were taken out.
 template <typename T, int DP>
-__device__ void exact_row(const AttnParams& p, int b, int hk, const T* q, int k0, int k1, float& m,
-                          float& l, float (&o)[DP / 32]) {
-  const int lane = lane_id();
-  m = -INFINITY;
-  l = 0.f;
+__device__ __forceinline__ void decide_rows(const AttnParams& p, const TileWork& w, int x, int tok, uint32_t o_tmem,
+                                            bool counts, int* state) {
+  constexpr int KT = TilesCfg<DP>::KT;
+  const int row0 = x * tok * p.G + (warp_id() & 3) * 32;  // of the item; the warp's first
+  const int rows = max(0, min(32, min((x + 1) * tok, w.count) * p.G - row0));
+  bool odd = false;
+#pragma unroll 1
+  for (int c = 0; c < DP / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld32(o_tmem + c * 32, o);
+    tmem_ld_wait();
 #pragma unroll
-  for (int c = 0; c < DP / 32; ++c) o[c] = 0.f;
-  auto row_of = [&](const void* pool, long long sp, long long sh, long long sr, int key) -> const T* {
-    const int page = clip_page(__ldg(p.table + b * p.table_stride + key / p.page_size), p.num_pages);
-    if (page == p.num_pages) return nullptr;  // zeros, as in the tiles
-    return static_cast<const T*>(pool) + page * sp + hk * sh + (key % p.page_size) * sr;
-  };
-  for (int j0 = k0; j0 < k1; j0 += 32) {
-    float s = -INFINITY;
-    if (j0 + lane < k1) {
-      const T* k = row_of(p.k, p.kp_p, p.kp_h, p.kp_r, j0 + lane);
-      float dot = 0.f;
-      if (k)
-        for (int d = 0; d < p.D; d += 2) {
-          const float2 x = unpack2<T>(*reinterpret_cast<const uint32_t*>(q + d));
-          const float2 y = unpack2<T>(*reinterpret_cast<const uint32_t*>(k + d));
-          dot = fmaf(x.x, y.x, dot);
-          dot = fmaf(x.y, y.y, dot);
-        }
-      s = dot * p.scale_log2;
-    }
-    float top = s;
-#pragma unroll
-    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    top = fmaxf(m, top);
-    const float a = part_weight(m, top);
-    const float e = s == -INFINITY ? 0.f : exp2f(s - top);
-    m = top;
-    float sum = e;
-#pragma unroll
-    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    l = l * a + sum;
-#pragma unroll
-    for (int c = 0; c < DP / 32; ++c) o[c] *= a;
-    for (int i = 0; i < min(32, k1 - j0); ++i) {
-      const float w = __shfl_sync(0xffffffffu, e, i);
-      const T* v = row_of(p.v, p.vp_p, p.vp_h, p.vp_r, j0 + i);
-      if (!v) continue;
-#pragma unroll
-      for (int c = 0; c < DP / 32; ++c)
-        if (lane + c * 32 < p.D) {
-          const uint32_t u = reinterpret_cast<const uint16_t*>(v)[lane + c * 32];
-          o[c] = fmaf(w, unpack2<T>(u).x, o[c]);
-        }
-    }
+    for (int k = 0; k < 32; ++k) odd |= !(fabsf(__uint_as_float(o[k])) < INFINITY);
   }
+  const int begin = w.tile0 * KT, end = begin + w.nt * KT;
+  int from = begin, to = end;  // keys of the item, or first those of its masked tiles at one end
+  const int low = min(end, (w.all_lo + KT - 1) / KT * KT), high = max(begin, w.all_hi / KT * KT);
+  const bool ends = !__any_sync(0xffffffffu, odd && counts) && low < high;
+  if (ends) to = low;
+  uint32_t marks[DP / 16] = {};
+#pragma unroll 1
+  while (true) {
+    mark_values<T, DP>(p, w.b, w.hk, w.s, w.first * p.G + row0, rows, from, to, marks, [&] { atomicAdd(state, 2); });
+    if (to == end) break;
+    from = high;
+    to = end;
+  }
+#pragma unroll 1
+  for (int c = 0; c < DP / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld32(o_tmem + c * 32, o);
+    tmem_ld_wait();
+#pragma unroll
+    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(marked<DP>(__uint_as_float(o[k]), marks, c * 32 + k));
+    tmem_st32(o_tmem + c * 32, o);
+  }
+  tmem_st_wait();
 }
 
 template <typename T, int DP>
@@ -216,7 +202,9 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
   uint64_t* ask = taken + 1;           // the item's loads are nearly all issued
   void* answer = taken + 2;            // 16 bytes, 16-byte aligned
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 4);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  // Bit 0: the kernel is given up; above it, counted up while values are gone over again.
+  int* state = reinterpret_cast<int*>(tmem_slot + 1);
+  const volatile int* watched = state;
   static_assert((4 * STAGES + 18) * 8 + 8 <= C::kBarBytes, "barrier area");
   static_assert((4 * STAGES + 16) % 2 == 0, "the answer is 16-byte aligned");
   const int warp = warp_id(), lane = lane_id();
@@ -242,7 +230,7 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
     }
     mbar_init(taken, 1);
     mbar_init(ask, 1);
-    *abort_flag = 0;
+    *state = 0;
     fence_barrier_init();
   }
   if (warp == 13) {
@@ -256,17 +244,22 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
 
   // Whole-warp wait; false if the kernel is to be given up: another role did,
   // or the limit ran out (`late` then tells that this warp is the first). The
-  // limit leaves room for rows that are formed one by one.
-  constexpr long long kLimit = 4 * kSpinLimitCycles;
+  // limit runs anew while softmax warps go over values again.
   bool ok = true, late = false;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    const long long t0 = clock64();
+    long long t0 = clock64();
+    int seen = 0;
     while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
-      if (*abort_flag) return false;
-      if (clock64() - t0 > kLimit) {
+      const int now = *watched;
+      if (now & 1) return false;
+      if (now != seen) {
+        seen = now;
+        t0 = clock64();
+      }
+      if (clock64() - t0 > kSpinLimitCycles) {
         late = true;
-        *abort_flag = 1;
+        atomicOr(state, 1);
         return false;
       }
     }
@@ -353,7 +346,7 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
         }
         if (ok) release_work();
       }
-      if (*abort_flag) {
+      if (*watched & 1) {
         wait_late(q_full, item & 1);
         for (int i = max(0, issued - STAGES); i < issued; ++i) wait_late(&full[i % STAGES], (i / STAGES) & 1);
       }
@@ -499,7 +492,7 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
           w.slot = entry * p.splits + split;
           w.all_hi = key_hi(p, s, w.first);
           w.all_lo = key_lo(p, s, w.first + w.count - 1);
-          w.by_hand = 0;
+          w.special = 0;
           live = split < w.pieces;
         }
         if (split == 0 && p.splits > 1 && lane == 0) {
@@ -653,7 +646,10 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
       const long long t = w.s.t0 + w.first + tr;
       const bool whole = w.pieces == 1;
       const long long part = static_cast<long long>(w.slot) * 256 + row;
-      if (!*reinterpret_cast<volatile int*>(&work[item & 1].by_hand)) {
+      const bool counts = valid && fabsf(l) < INFINITY;
+      // due: values of the item's keys that are not finite are to be brought into O
+      bool due = *reinterpret_cast<volatile int*>(&work[item & 1].special) != 0, decided = false;
+      {
         // Through shared memory, 128 bytes of each of the warp's 32 rows at a
         // time (16-byte chunks swizzled by row), so that rows leave as whole
         // 128-byte lines: lane 8 q + c has chunk c of rows q, q + 4, ...
@@ -669,12 +665,22 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
         const int row_bytes = whole ? p.D * 2 : DP * 4;
 #pragma unroll 1
         for (int c0 = 0; c0 < (whole ? DP / 64 : DP / 32); ++c0) {
+          if (due) {
+            decide_rows<T, DP>(p, w, x, tok, o_tmem, counts, state);
+            due = false;
+            decided = true;
+          }
           uint32_t o[32];
+          const uint64_t zero = f2_pack(0.f, 0.f);
+          uint64_t odd = zero;  // 0, NaN where a value is not finite
           if (whole) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               tmem_ld32(o_tmem + c0 * 64 + half * 32, o);
               tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 32; k += 2)
+                odd = f2_fma(f2_pack(__uint_as_float(o[k]), __uint_as_float(o[k + 1])), zero, odd);
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 uint4 v;
@@ -689,9 +695,19 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
             tmem_ld32(o_tmem + c0 * 32, o);
             tmem_ld_wait();
 #pragma unroll
+            for (int k = 0; k < 32; k += 2)
+              odd = f2_fma(f2_pack(__uint_as_float(o[k]), __uint_as_float(o[k + 1])), zero, odd);
+#pragma unroll
             for (int k = 0; k < 8; ++k)
               *reinterpret_cast<uint4*>(stage + lane * 128 + ((k ^ (lane & 7)) << 4)) =
                   make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          }
+          float n0, n1;
+          f2_unpack(odd, n0, n1);
+          if (!decided && __any_sync(0xffffffffu, counts && n0 + n1 != 0.f)) {
+            due = true;
+            --c0;  // once more
+            continue;
           }
           __syncwarp();
           uint4 v[8];
@@ -711,30 +727,6 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
           if (!whole) p.part_ml[part] = make_float2(m, l);
           else if (p.lse) p.lse[t * p.Hq + h] = log_sum(m, l);
         }
-      } else {
-        const int row0 = x * tok * p.G + (warp & 3) * 32;
-        for (int rr = row0; rr < min(row0 + 32, min((x + 1) * tok, w.count) * p.G); ++rr) {
-          const int tk = w.first + rr / p.G, hh = w.hk * p.G + rr % p.G;
-          const long long tt = w.s.t0 + tk;
-          float me, le, o[DP / 32];
-          exact_row<T, DP>(p, w.b, w.hk, static_cast<const T*>(p.q) + tt * p.qs_t + hh * p.qs_h,
-                           max(w.tile0 * KT, key_lo(p, w.s, tk)),
-                           min((w.tile0 + w.nt) * KT, key_hi(p, w.s, tk)), me, le, o);
-          const long long at = static_cast<long long>(w.slot) * 256 + rr;
-          const float inv = inverse_sum(le);
-#pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            const int d = lane + c * 32;
-            if (!whole) p.part_o[at * DP + d] = o[c];
-            else if (d < p.D)
-              reinterpret_cast<uint16_t*>(static_cast<T*>(p.out) + tt * p.os_t + hh * p.os_h)[d] =
-                  static_cast<uint16_t>(pack2<T>(o[c] * inv, 0.f));
-          }
-          if (lane == 0) {
-            if (!whole) p.part_ml[at] = make_float2(me, le);
-            else if (p.lse) p.lse[tt * p.Hq + hh] = log_sum(me, le);
-          }
-        }
       }
       tc_fence_before();
       release_work();
@@ -742,8 +734,8 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
   } else {
     // ---------------------------------------------- values of masked tiles --
     // 0 * inf and 0 * NaN are NaN: value rows past the sequence's end (stale
-    // memory) are cleared; where another masked value is not finite, the item's
-    // rows are formed one by one instead.
+    // memory) are cleared, and other values of masked tiles that are not finite
+    // taken out: the rows that see them get them with the output.
     setmaxnreg_dec<C::kRegsValues>();
     const int t = static_cast<int>(threadIdx.x) - 256;
     uint32_t place = 0, looked = 0;  // looked: phases of v_look, a bit per stage
@@ -767,11 +759,16 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const int key = k * 16 + (t >> 3);
-            if (key < live) bad |= not_finite4<T>(u[k]);
-            else *reinterpret_cast<uint4*>(v + c * (KT * 128) + (k * 128 + t) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            uint4* at16 = reinterpret_cast<uint4*>(v + c * (KT * 128) + (k * 128 + t) * 16);
+            if (key >= live) {
+              *at16 = make_uint4(0u, 0u, 0u, 0u);
+            } else if (not_finite4<T>(u[k])) {
+              *at16 = finite_only4<T>(u[k]);
+              bad = 1;
+            }
           }
         }
-        if (bad) *reinterpret_cast<volatile int*>(&work[item & 1].by_hand) = 1;
+        if (bad) *reinterpret_cast<volatile int*>(&work[item & 1].special) = 1;
         fence_proxy_async_smem();
         mbar_arrive(&v_fixed[st]);
       }

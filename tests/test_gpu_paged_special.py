@@ -6,7 +6,7 @@ import math
 
 import pytest
 
-from tests.test_gpu_paged_attention import ROWS, definition, make
+from tests.test_gpu_paged_attention import ROWS, TILES, definition, make
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -50,7 +50,8 @@ def spoil(vp, table, new, total, page, places):
 
 @pytest.mark.parametrize("places", [[0.0], [0.4], [0.97], [0.1, 0.5, 0.999]], ids=str)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("case", [ROWS[1], ROWS[2], ROWS[4], ROWS[5], ROWS[7], ROWS[8], ROWS[11]], ids=str)
+@pytest.mark.parametrize("case", [ROWS[1], ROWS[2], ROWS[4], ROWS[5], ROWS[7], ROWS[8], ROWS[9], ROWS[11],
+                                  TILES[1], TILES[2], TILES[4], TILES[5], TILES[6], TILES[8], TILES[9]], ids=str)
 def test_infinite_values(ops, case, dtype, places):
     q, kp, vp, table, cu, lens = args = make(*case, dtype)
     spoil(vp, table, case[0], case[1], case[2], places)
@@ -63,8 +64,8 @@ def test_infinite_values(ops, case, dtype, places):
         compare(lse[:n], wl[:n], ltol[:n])
 
 
-@pytest.mark.parametrize("max_q_len", [1])
-@pytest.mark.parametrize("case", [ROWS[4], ROWS[5], ROWS[11]], ids=str)
+@pytest.mark.parametrize("max_q_len", [None, 1])
+@pytest.mark.parametrize("case", [ROWS[4], ROWS[5], ROWS[11], TILES[4]], ids=str)
 def test_infinite_values_windows_and_any_kernel(ops, case, max_q_len):
     q, kp, vp, table, cu, lens = args = make(*case, torch.bfloat16)
     spoil(vp, table, case[0], case[1], case[2], [0.0, 0.93, 0.98])
@@ -76,7 +77,7 @@ def test_infinite_values_windows_and_any_kernel(ops, case, max_q_len):
         compare(lse[:n], wl[:n], ltol[:n])
 
 
-@pytest.mark.parametrize("case", [ROWS[1], ROWS[4], ROWS[11]], ids=str)
+@pytest.mark.parametrize("case", [ROWS[1], ROWS[4], ROWS[11], TILES[2], TILES[4]], ids=str)
 def test_infinite_keys_and_values(ops, case):
     """A key that scores -inf has weight 0, and 0 * inf is NaN; one that scores
     inf leaves its rows NaN."""
@@ -96,7 +97,7 @@ def test_infinite_keys_and_values(ops, case):
 
 def test_queries_that_are_not_finite(ops):
     """A row whose scores are NaN is NaN, and no other."""
-    for case in (ROWS[4], ROWS[5]):
+    for case in (ROWS[4], TILES[4]):
         args = make(*case, torch.bfloat16)
         args[0][1] = float("nan")
         n = sum(case[0])
@@ -104,3 +105,35 @@ def test_queries_that_are_not_finite(ops):
         out, lse = ops.paged_attention(*args, max_q_len=max(case[0]), return_lse=True)
         compare(out[:n], want[:n], tol[:n])
         compare(lse[:n], wl[:n], ltol[:n])
+
+
+def test_one_infinite_value_in_a_long_context(ops):
+    """The last of many new tokens has an infinite value: its column is infinite
+    for that token alone, and finding that out takes no more than going over the
+    values again (a row formed key by key would take hundreds of times the call's own time)."""
+    case = ([256], [30000], 64, 32, 1, 128)
+    q, kp, vp, table, cu, lens = args = make(*case, torch.bfloat16, pad=0)
+    last = 29999
+    at = table[0, last // 64], 3, last % 64, 17
+
+    def run():
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        start.record()
+        out = ops.paged_attention(*args, max_q_len=256)
+        end.record()
+        end.synchronize()
+        return out, start.elapsed_time(end)
+
+    clean, _ = run()
+    usual = min(run()[1] for _ in range(3))
+    vp[at] = math.inf
+    out, _ = run()
+    longer = min(run()[1] for _ in range(3))
+    want = clean.clone()
+    want[255, 3, 17] = math.inf
+    # (in that tile the value was part of no sum, so all others are as they were but
+    # for the clean value's own share)
+    same = out == want
+    same[255, 3, 17] = bool(out[255, 3, 17] == math.inf)
+    assert bool(same.all())
+    assert longer < 20 * usual, (longer, usual)
