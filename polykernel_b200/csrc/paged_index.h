@@ -43,12 +43,15 @@ PKB_INDEX int clip_lo(const Seq& s, int i, int window) {
   return window && s.pos0 + i >= window ? s.pos0 + i - window + 1 : 0;  // (no step leaves 32 bits)
 }
 
-// Key tiles of `kt` keys that the tokens [first, last] need, from tile0 on: at
-// least one, which may be masked throughout, so that rows without keys take the
-// common path.
+// Key tiles of `kt` keys that hold the keys [lo, hi), from tile0 on: at least one,
+// which may be masked throughout, so that rows without keys take the common path.
+PKB_INDEX int tiles_of_keys(int lo, int hi, int kt, int& tile0) {
+  tile0 = lo / kt;
+  return most(1, (hi - tile0 * kt + kt - 1) / kt);
+}
+// Those that the tokens [first, last] need.
 PKB_INDEX int clip_tiles(const Seq& s, int first, int last, int causal, int window, int kt, int& tile0) {
-  tile0 = clip_lo(s, first, window) / kt;
-  return most(1, (clip_hi(s, last, causal) - tile0 * kt + kt - 1) / kt);
+  return tiles_of_keys(clip_lo(s, first, window), clip_hi(s, last, causal), kt, tile0);
 }
 
 // A page of the pool, or num_pages (past its end, where tensor-map reads give

@@ -109,29 +109,36 @@ struct RowCursor {
   int b, hk, rt;
   Seq s;
   int rows, row_tiles;  // rows of the sequence
-  int tile0, n;         // key tiles of this row tile
+  int seen_lo, seen_hi; // keys that some row of this row tile sees
+  int tile0, n;         // its key tiles
 
   __device__ explicit RowCursor(const AttnParams& p_) : p(p_) {}
   __device__ static int rows_of(const AttnParams& p, const Seq& s) {
     const int rows = s.nq * p.G;
     return rows >= p.min_rows && rows <= p.max_rows ? rows : 0;
   }
-  __device__ static int tiles_of(const AttnParams& p, const Seq& s, int rows, int rt, int& tile0) {
-    if (rows <= MR) return key_tiles<64>(p, s, 0, s.nq - 1, tile0);
-    return key_tiles<64>(p, s, rt * MR / p.G, (min(rows, rt * MR + MR) - 1) / p.G, tile0);
+  // Tokens of the row tile, the first and the last.
+  __device__ static int first_of(const AttnParams& p, int rows, int rt) { return rows <= MR ? 0 : rt * MR / p.G; }
+  __device__ static int last_of(const AttnParams& p, const Seq& s, int rows, int rt) {
+    return rows <= MR ? s.nq - 1 : (min(rows, rt * MR + MR) - 1) / p.G;
   }
   // Key tiles of a whole sequence (one key head).
   __device__ static long long units_of(const AttnParams& p, const Seq& s) {
     const int rows = rows_of(p, s);
     long long n = 0;
     int tile0;
-    for (int rt = 0; rt * MR < rows; ++rt) n += tiles_of(p, s, rows, rt, tile0);
+    for (int rt = 0; rt * MR < rows; ++rt) n += key_tiles<64>(p, s, first_of(p, rows, rt), last_of(p, s, rows, rt), tile0);
     return n;
   }
   __device__ void load() {
     s = load_seq(p, b);
     rows = rows_of(p, s);
     row_tiles = (rows + MR - 1) / MR;
+  }
+  __device__ void set_tiles() {
+    seen_lo = key_lo(p, s, first_of(p, rows, rt));
+    seen_hi = key_hi(p, s, last_of(p, s, rows, rt));
+    n = tiles_of_keys(seen_lo, seen_hi, 64, tile0);
   }
   // Start in sequence b, `rem` key tiles after its first one; returns the
   // offset within the row tile.
@@ -142,7 +149,7 @@ struct RowCursor {
     hk = static_cast<int>(divide(rem, per_head));
     rem -= hk * per_head;
     for (rt = 0;; ++rt) {
-      n = tiles_of(p, s, rows, rt, tile0);
+      set_tiles();
       if (rem < n) return static_cast<int>(rem);
       rem -= n;
     }
@@ -158,7 +165,7 @@ struct RowCursor {
         } while (rows == 0);
       }
     }
-    n = tiles_of(p, s, rows, rt, tile0);
+    set_tiles();
   }
 };
 
@@ -244,9 +251,11 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
     }
     for (long long u = u0; u < u1 && ok;) {
       const int run = static_cast<int>(min(static_cast<long long>(at.n - off), u1 - u));
+      // Keys that no row of the tile sees are not looked up: pages behind a
+      // window may be gone.
       auto lookup = [&](int tile) {  // this lane's page in that key tile
         const int key = (at.tile0 + tile) * KT + bx * p.box;
-        return mine && key < at.s.len ? page_of(p, at.b, key) : -1;
+        return mine && key + p.box > at.seen_lo && key < at.seen_hi ? page_of(p, at.b, key) : -1;
       };
       int page = lookup(off);
       for (int i = 0; i < run && ok; ++i) {
@@ -434,14 +443,15 @@ __global__ void __launch_bounds__(RowsCfg<DP, MR>::kThreads, RowsCfg<DP, MR>::kB
       if (!ok) break;
       const uint32_t base = slots_addr + slot * C::SLOT;
       if (masked) {
-        // A masked key has P = 0, but 0 * inf and 0 * NaN are NaN. Rows past
-        // the sequence's end (stale memory) are cleared here, and values that are not
-        // finite taken out: the rows that see them get them at the end.
+        // A masked key has P = 0, but 0 * inf and 0 * NaN are NaN. Rows that no
+        // row sees (stale memory, or not fetched) are cleared here, and values that
+        // are not finite taken out: the rows that see them get them at the end.
+        const int seen_lo = at.seen_lo - key0, seen_hi = at.seen_hi - key0;
         bool bad = false;
         for (int x = lane; x < KW * HALVES * 8; x += 32) {
           const int key = wk * KW + x / (HALVES * 8), c = x % (HALVES * 8);
           uint4* w = reinterpret_cast<uint4*>(smem + slot * C::SLOT + (c >> 3) * (KT * 128) + key * 128 + (c & 7) * 16);
-          if (key0 + key >= at.s.len) {
+          if (key < seen_lo || key >= seen_hi) {
             *w = make_uint4(0u, 0u, 0u, 0u);
           } else if (not_finite4<T>(*w)) {
             *w = finite_only4<T>(*w);

@@ -15,8 +15,8 @@
 //                    row's maximum moved by more than 2^8 (P stays below 2^8 and
 //                    the sums share the stale maximum, so the quotient is
 //                    exact), and writes the output.
-//   warps 8-11       clear value rows past the end of a sequence and take values
-//                    that are not finite out of tiles that some row masks.
+//   warps 8-11       in tiles that some row masks: clear value rows that no row
+//                    sees and take values that are not finite out of the others.
 //   warp 12          TMA: Q, and key and value pages into one ring.
 //   warp 13          MMA issue, and owner of TMEM.
 //   warp 14          work: blocks stay resident and take over the work of blocks
@@ -304,9 +304,11 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
       while (ok && next_work()) {
         const TileWork w = work[item & 1];
         const bool two = w.count > tok;
+        // (not for keys that no row of the item sees: pages behind a window may be gone)
+        const int seen_lo = key_lo(p, w.s, w.first), seen_hi = key_hi(p, w.s, w.first + w.count - 1);
         auto lookup = [&](int j) {
           const int key = (w.tile0 + j) * KT + bx * p.box;
-          return mine && key < w.s.len ? page_of(p, w.b, key) : -1;
+          return mine && key + p.box > seen_lo && key < seen_hi ? page_of(p, w.b, key) : -1;
         };
         int page = lookup(0);
         for (int j = 0; j < w.nt && ok; ++j) {
@@ -733,14 +735,15 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
     }
   } else {
     // ---------------------------------------------- values of masked tiles --
-    // 0 * inf and 0 * NaN are NaN: value rows past the sequence's end (stale
-    // memory) are cleared, and other values of masked tiles that are not finite
+    // 0 * inf and 0 * NaN are NaN: value rows that no row of the item sees (stale
+    // memory, or not fetched) are cleared, and other values of masked tiles that are not finite
     // taken out: the rows that see them get them with the output.
     setmaxnreg_dec<C::kRegsValues>();
     const int t = static_cast<int>(threadIdx.x) - 256;
     uint32_t place = 0, looked = 0;  // looked: phases of v_look, a bit per stage
     while (ok && next_work()) {
       const TileWork w = work[item & 1];
+      const int seen_lo = key_lo(p, w.s, w.first), seen_hi = key_hi(p, w.s, w.first + w.count - 1);
       for (int j = 0; j < w.nt && ok; ++j, place += 2) {
         if (!masked(w, j)) continue;
         const uint32_t at = place + 1, st = at % STAGES;
@@ -749,7 +752,7 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
         if (!ok) break;
         looked ^= 1u << st;
         uint8_t* v = smem + C::OFF_KV + st * C::TILE;
-        const int live = w.s.len - (w.tile0 + j) * KT;  // key rows of the sequence
+        const int key0 = (w.tile0 + j) * KT, live_lo = seen_lo - key0, live_hi = seen_hi - key0;
         uint32_t bad = 0;
 #pragma unroll
         for (int c = 0; c < C::HALVES; ++c) {
@@ -760,7 +763,7 @@ __global__ void __launch_bounds__(TilesCfg<DP>::kThreads, 1)
           for (int k = 0; k < 8; ++k) {
             const int key = k * 16 + (t >> 3);
             uint4* at16 = reinterpret_cast<uint4*>(v + c * (KT * 128) + (k * 128 + t) * 16);
-            if (key >= live) {
+            if (key < live_lo || key >= live_hi) {
               *at16 = make_uint4(0u, 0u, 0u, 0u);
             } else if (not_finite4<T>(u[k])) {
               *at16 = finite_only4<T>(u[k]);

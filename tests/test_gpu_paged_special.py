@@ -137,3 +137,32 @@ def test_one_infinite_value_in_a_long_context(ops):
     same[255, 3, 17] = bool(out[255, 3, 17] == math.inf)
     assert bool(same.all())
     assert longer < 20 * usual, (longer, usual)
+
+
+@pytest.mark.parametrize("gone", [-1, 2 ** 31 - 1])
+@pytest.mark.parametrize("window", [1, 40, 200])
+@pytest.mark.parametrize("case", [ROWS[1], ROWS[4], ROWS[5], ROWS[8], ROWS[10], ROWS[11], TILES[4], TILES[5],
+                                  TILES[6], TILES[8]], ids=str)
+def test_pages_behind_the_window_may_be_gone(ops, case, window, gone):
+    """A server that frees pages which no new token's window reaches marks them in
+    the table: that is no error, and changes nothing (the fixture checks the error word)."""
+    q, kp, vp, table, cu, lens = args = make(*case, torch.bfloat16)
+    n, page = sum(case[0]), case[2]
+    freed = table.clone()
+    for b, (c, t) in enumerate(zip(case[0], case[1])):
+        freed[b, :max(0, t - c - window + 1) // page] = gone
+    kw = dict(max_q_len=max(case[0]), window=window, return_lse=True)
+    out, lse = ops.paged_attention(q, kp, vp, freed, cu, lens, **kw)
+    want, wl, tol, ltol = definition(*args, window=window)
+    compare(out[:n], want[:n], tol[:n])
+    compare(lse[:n], wl[:n], ltol[:n])
+
+
+@pytest.mark.parametrize("case", [ROWS[4], TILES[4]], ids=str)
+def test_pages_that_the_window_reaches_may_not(ops, case):
+    import polykernel_b200 as pk
+    q, kp, vp, table, cu, lens = make(*case, torch.bfloat16)
+    c, t, page = case[0][2], case[1][2], case[2]
+    table[2, max(0, t - c - 100 + 1) // page] = -1
+    ops.paged_attention(q, kp, vp, table, cu, lens, max_q_len=max(case[0]), window=100)
+    assert pk.device_error() == 8
