@@ -10,6 +10,7 @@
 #include <optional>
 
 #include "../../include/pkb200.h"
+#include "overlap.h"
 
 namespace py = pybind11;
 using at::Tensor;
@@ -59,10 +60,21 @@ void check_rows(const Tensor& t, const char* name, at::ScalarType type, const at
   if (t.sizes() != shape) bad_value(name, " must have shape ", shape, ", got ", t.sizes());
   check_last(t, name);
 }
-// `out` may be the input itself, but no other view of its memory.
-void check_in_place(const Tensor& out, const char* name, const Tensor& in) {
-  if (out.data_ptr() == in.data_ptr() && out.strides() != in.strides())
-    bad_value(name, " may be the input itself, not another view of its memory");
+pkb200::View view_of(const Tensor& t) {
+  pkb200::View v{reinterpret_cast<std::uintptr_t>(t.data_ptr()), static_cast<int>(t.dim()), {}, {},
+                 static_cast<long long>(t.element_size())};
+  for (int i = 0; i < v.axes; ++i) {
+    v.n[i] = t.size(i);
+    v.stride[i] = t.stride(i) * v.size;
+  }
+  return v;
+}
+// What is written must not share memory with what is read or written beside it;
+// `itself`: but may be the very same tensor.
+void check_apart(const Tensor& out, const char* name, const Tensor& other, const char* other_name, bool itself = false) {
+  const pkb200::View a = view_of(out), b = view_of(other);
+  if (itself && a.same_places(b)) return;
+  if (pkb200::share_memory(a, b)) bad_value(name, " overlaps ", other_name);
 }
 // Memory that is written must not be one place under several indexes.
 void check_written(const Tensor& t, const char* name) {
@@ -123,7 +135,7 @@ Tensor rope(const Tensor& x, const Tensor& positions, const Tensor& inv_freq, bo
   if (out) {
     y = *out;
     check_rows(y, "out", x.scalar_type(), dev, x.sizes());
-    check_in_place(y, "out", x);
+    check_apart(y, "out", x, "x", true);
     check_written(y, "out");
   } else {
     y = at::empty(x.sizes(), x.options());
@@ -232,11 +244,20 @@ py::object paged_kv_append(const Tensor& k, const Tensor& v, const Tensor& k_pag
     if (q_out) {
       rotated = *q_out;
       check_rows(rotated, "q_out", type, p.device, q->sizes());
-      check_in_place(rotated, "q_out", *q);
+      check_apart(rotated, "q_out", *q, "q", true);
+      check_apart(rotated, "q_out", k, "k");
+      check_apart(rotated, "q_out", v, "v");
       check_written(rotated, "q_out");
     } else {
       rotated = at::empty(q->sizes(), q->options());
     }
+  }
+  check_apart(v_pages, "v_pages", k_pages, "k_pages");
+  for (const auto& [pool, name] : {std::pair<const Tensor&, const char*>{k_pages, "k_pages"}, {v_pages, "v_pages"}}) {
+    check_apart(pool, name, k, "k");
+    check_apart(pool, name, v, "v");
+    if (q) check_apart(pool, name, *q, "q");
+    if (q) check_apart(pool, name, rotated, "q_out");
   }
   const RowStrides ks(k), vs(v), qs(q ? *q : k), os(q ? rotated : k);
   check_status(pkb200_paged_kv_append(&p.cache, &p.batch, k.data_ptr(), ks.s, v.data_ptr(), vs.s,
@@ -279,6 +300,9 @@ py::object paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor&
     check_rows(out, "out", q.scalar_type(), p.device, q.sizes());
     check_aligned(out, "out");
     check_written(out, "out");
+    check_apart(out, "out", q, "q", true);
+    check_apart(out, "out", k_pages, "k_pages");
+    check_apart(out, "out", v_pages, "v_pages");
   } else {
     out = at::empty(q.sizes(), q.options());
   }

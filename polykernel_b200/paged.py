@@ -113,7 +113,7 @@ def rope(x, positions, inv_freq, interleaved=False, factor=1.0, out=None):
     2 * len(inv_freq) values of a head are rotated in pairs (i, half + i), or
     (2i, 2i + 1) if interleaved, by position * inv_freq[i], and scaled by factor;
     the others are copied. Angles are exact for positions up to 2^31. `out` may
-    be x."""
+    be x, and otherwise shares no memory with it."""
     return load_paged().rope(x, positions, inv_freq, interleaved, factor, out, False)
 
 
@@ -142,7 +142,8 @@ def paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, seq_lens, max_q
     reads key head h // (q_heads / heads). With `causal` a token sees the keys up to
     its own position, with `window` the last `window` of those. A row that sees no
     key gives zeros (and -inf). Returns out, or (out, lse) with return_lse, the
-    fp32 [T, q_heads] logarithms of the sums of exponentials; both can be passed in.
+    fp32 [T, q_heads] logarithms of the sums of exponentials; both can be passed in
+    (out may be q, and otherwise shares no memory with the inputs).
     Rows of no sequence keep what `out` and `lse` held.
 
     dim and the page size are multiples of 8, dim at most 256. max_q_len, the most
