@@ -13,7 +13,8 @@ here synchronises, and a captured graph follows the tensors' contents. Rows from
 cu_seqlens[-1] on belong to no sequence and are left as they were.
 
 Tensors are bf16 or fp16 (`rope`: also fp32), strided as they come out of a
-fused projection, with a contiguous last axis.
+fused projection, with a contiguous last axis. `rope` is differentiable; through
+a cache (`paged_kv_append`, `paged_attention`) no gradient flows.
 """
 from __future__ import annotations
 
@@ -107,20 +108,49 @@ def rope_frequencies(rot_dim, base=10000.0, scaling=None, device="cuda"):
     return f.float().to(device), float(factor)
 
 
+class _Rope(torch.autograd.Function):
+    """`rope` (or `rope_backward`) as a step of autograd. The map is linear, and
+    each of the two is the other's gradient."""
+
+    @staticmethod
+    def forward(ctx, x, positions, inv_freq, interleaved, factor, backward):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.how = interleaved, factor, backward
+        return load_paged().rope(x, positions, inv_freq, interleaved, factor, None, backward)
+
+    @staticmethod
+    def backward(ctx, grad):
+        interleaved, factor, backward = ctx.how
+        if grad.stride(-1) != 1:  # a sum's gradient is expanded
+            grad = grad.contiguous()
+        return _Rope.apply(grad, *ctx.saved_tensors, interleaved, factor, not backward), None, None, None, None, None
+
+
+def _rope(x, positions, inv_freq, interleaved, factor, out, backward):
+    if torch.is_grad_enabled() and (x.requires_grad or inv_freq.requires_grad):
+        if inv_freq.requires_grad:
+            raise ValueError("inv_freq gets no gradient: pass inv_freq.detach()")
+        if out is not None:
+            raise ValueError("out is not taken for a tensor that requires a gradient")
+        return _Rope.apply(x, positions, inv_freq, interleaved, factor, backward)
+    return load_paged().rope(x, positions, inv_freq, interleaved, factor, out, backward)
+
+
 def rope(x, positions, inv_freq, interleaved=False, factor=1.0, out=None):
     """Rotary positions. x is [T, H, D] (packed tokens) or [B, H, S, D] (what
     `qkv_projection` returns); positions int64 [T], [S] or [B, S]. The first
     2 * len(inv_freq) values of a head are rotated in pairs (i, half + i), or
     (2i, 2i + 1) if interleaved, by position * inv_freq[i], and scaled by factor;
-    the others are copied. Angles are exact for positions up to 2^31. `out` may
-    be x, and otherwise shares no memory with it."""
-    return load_paged().rope(x, positions, inv_freq, interleaved, factor, out, False)
+    the others are copied. Angles are formed in 64 bits and are within
+    2^-20 radians for |position * inv_freq| up to 2^31. `out` may be x, and otherwise shares no memory with it.
+    Differentiable with respect to x (without `out`)."""
+    return _rope(x, positions, inv_freq, interleaved, factor, out, False)
 
 
 def rope_backward(grad, positions, inv_freq, interleaved=False, factor=1.0, out=None):
     """The gradient of `rope` with respect to x, from that of its result: the
     rotation by the negative angles (arguments as for `rope`)."""
-    return load_paged().rope(grad, positions, inv_freq, interleaved, factor, out, True)
+    return _rope(grad, positions, inv_freq, interleaved, factor, out, True)
 
 
 def paged_kv_append(k, v, k_pages, v_pages, page_table, cu_seqlens, seq_lens, inv_freq=None,
