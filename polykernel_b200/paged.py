@@ -18,11 +18,11 @@ a cache (`paged_kv_append`, `paged_attention`) no gradient flows.
 """
 from __future__ import annotations
 
-import glob
 import importlib.machinery
 import importlib.util
 import math
 import os
+import sysconfig
 
 import torch
 
@@ -36,12 +36,13 @@ def load_paged():
     global _module
     if _module is None:
         lib()  # the library that it calls
-        found = glob.glob(os.path.join(os.path.dirname(LIB_PATH), "_paged.*.so"))
-        if not found:
+        # (built per Python version: another one's module beside it is not this one's)
+        path = os.path.join(os.path.dirname(LIB_PATH), "_paged" + sysconfig.get_config_var("EXT_SUFFIX"))
+        if not os.path.exists(path):
             raise RuntimeError("pkb200: Python module of the paged operators not built; run "
                                "`python -c 'import __graft_entry__ as g; g.build()'`")
-        loader = importlib.machinery.ExtensionFileLoader("_paged", found[0])
-        spec = importlib.util.spec_from_file_location("_paged", found[0], loader=loader)
+        loader = importlib.machinery.ExtensionFileLoader("_paged", path)
+        spec = importlib.util.spec_from_file_location("_paged", path, loader=loader)
         module = importlib.util.module_from_spec(spec)
         loader.exec_module(module)
         _module = module
