@@ -1,5 +1,6 @@
-"""CPU: the compiled module of the paged operators is found by its exact name."""
+"""CPU: how the compiled module of the paged operators is built and found."""
 import os
+import subprocess
 import sysconfig
 
 import pytest
@@ -17,3 +18,12 @@ def test_only_this_pythons_module_is_loaded(tmp_path, monkeypatch):
     for name in (here, "libpkb200.so"):
         os.symlink(os.path.join(os.path.dirname(_lib.LIB_PATH), name), tmp_path / name)
     assert hasattr(paged.load_paged(), "rope")
+
+
+def test_the_library_builds_without_python(tmp_path):
+    """`make` in csrc needs nvcc alone: its default target runs no Python."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "polykernel_b200", "csrc")
+    plan = subprocess.run(["make", "-C", csrc, "-n", "-B"], capture_output=True, text=True, check=True).stdout
+    assert "nvcc" in plan and "python" not in plan
+    plan = subprocess.run(["make", "-C", csrc, "-n", "-B", "binding"], capture_output=True, text=True, check=True).stdout
+    assert "build_binding" in plan
