@@ -2,7 +2,7 @@
 import pytest
 
 from tests.test_gpu_paged_attention import ROWS, TILES, make
-from tests.test_gpu_rope_append import batch, gen
+from tests.test_gpu_rope_append import batch, check_rotated, gen
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -87,3 +87,24 @@ def test_attention_in_place_of_q(ops, case):
     want = ops.paged_attention(q, *rest, max_q_len=max(case[0]))[:n].clone()
     assert ops.paged_attention(q, *rest, max_q_len=max(case[0]), out=q) is q
     assert torch.equal(q[:n], want)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_append_with_a_factor(ops, dtype, interleaved):
+    """The factor on cos and sin reaches k and q in the cache's append."""
+    new, total, page = [3, 1], [20, 70], 16
+    table, cu, lens, pages = batch(new, total, page)
+    g = gen(8)
+    q, k, v = (torch.randn(4, h, 96, device="cuda", generator=g).to(dtype) for h in (6, 2, 2))
+    kp, vp = (torch.zeros(pages, 2, page, 96, device="cuda", dtype=dtype) for _ in range(2))
+    freq, factor = ops.rope_frequencies(64, scaling={"type": "yarn", "factor": 8.0, "original_length": 64})
+    assert factor > 1.2
+    got = ops.paged_kv_append(k, v, kp, vp, table, cu, lens, inv_freq=freq, interleaved=interleaved, factor=factor, q=q)
+    pos = torch.tensor([17, 18, 19, 69], device="cuda")
+    at = table[[0, 0, 0, 1], pos // page].long(), slice(None), pos % page
+    angle = pos.double()[:, None, None] * freq.double()
+    check_rotated(got, q, angle, interleaved, factor)
+    check_rotated(kp[at], k, angle, interleaved, factor)
+    assert torch.equal(got[..., 64:], q[..., 64:]) and torch.equal(kp[at][..., 64:], k[..., 64:])
+    assert torch.equal(vp[at], v)

@@ -166,3 +166,15 @@ def test_pages_that_the_window_reaches_may_not(ops, case):
     table[2, max(0, t - c - 100 + 1) // page] = -1
     ops.paged_attention(q, kp, vp, table, cu, lens, max_q_len=max(case[0]), window=100)
     assert pk.device_error() == 8
+
+
+@pytest.mark.parametrize("case", ROWS + TILES, ids=str)
+def test_log_sums(ops, case):
+    """Log-sums are finite where the definition's are (a NaN would pass a
+    comparison that leaves NaN out), for every shape."""
+    args = make(*case, torch.bfloat16)
+    n = sum(case[0])
+    want, wl, tol, ltol = definition(*args)
+    out, lse = ops.paged_attention(*args, max_q_len=max(case[0]), return_lse=True)
+    compare(lse[:n], wl[:n], ltol[:n])
+    compare(out[:n], want[:n], tol[:n])
