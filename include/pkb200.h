@@ -333,7 +333,10 @@ int pkb200_paged_kv_append(const pkb200_paged_cache* cache, const pkb200_paged_b
  * hold. dim a multiple of 8 up to 256, page_size a multiple of 8, base addresses
  * 16-byte aligned and strides multiples of 8 values; scale > 0.
  * max_q_len: the most new tokens of a sequence. It selects kernels (few rows
- * per key head, or many) and never changes what is computed.
+ * per key head, or many): any value is right for any batch, but the kernels round
+ * differently (up to 32 rows per key head the weights enter the product with v in
+ * two 16-bit terms, above that in one), so the last bits of a row depend on it
+ * and on the sizes of the batch. A call with the same arguments repeats itself.
  * workspace: caller-owned device memory, 256-byte aligned, of
  * pkb200_paged_attention_workspace_size bytes for the same arguments; calls that may
  * overlap on the GPU need their own. */

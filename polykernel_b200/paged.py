@@ -178,8 +178,10 @@ def paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, seq_lens, max_q
     Rows of no sequence keep what `out` and `lse` held.
 
     dim and the page size are multiples of 8, dim at most 256. max_q_len, the most
-    new tokens of any sequence, selects kernels and changes no result: pass it for
-    speed (by default 1 for as many tokens as sequences, T otherwise).
+    new tokens of any sequence, selects kernels: pass it for speed (by default 1 for
+    as many tokens as sequences, T otherwise). Any value is right for any batch, but
+    the kernels round differently, so the last bits of a row depend on it and on the
+    sizes of the batch. A call with the same arguments repeats itself.
     `workspace`: a uint8 tensor to use instead of a new one, if it is large enough;
     calls that may overlap need their own."""
     return load_paged().paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, seq_lens, max_q_len, causal,
