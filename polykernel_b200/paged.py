@@ -128,7 +128,7 @@ class _Rope(torch.autograd.Function):
 
 
 def _rope(x, positions, inv_freq, interleaved, factor, out, backward):
-    if torch.is_grad_enabled() and (x.requires_grad or inv_freq.requires_grad):
+    if torch.is_grad_enabled() and (getattr(x, "requires_grad", False) or getattr(inv_freq, "requires_grad", False)):
         if inv_freq.requires_grad:
             raise ValueError("inv_freq gets no gradient: pass inv_freq.detach()")
         if out is not None:

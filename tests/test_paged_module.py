@@ -27,3 +27,14 @@ def test_the_library_builds_without_python(tmp_path):
     assert "nvcc" in plan and "python" not in plan
     plan = subprocess.run(["make", "-C", csrc, "-n", "-B", "binding"], capture_output=True, text=True, check=True).stdout
     assert "build_binding" in plan
+
+
+@pytest.mark.parametrize("name", ["rope", "rope_backward"])
+def test_what_is_no_tensor_is_a_type_error(name):
+    torch = pytest.importorskip("torch")
+    from polykernel_b200 import ops
+    call = getattr(ops, name)
+    x, pos, f = torch.zeros(2, 1, 8), torch.zeros(2, dtype=torch.int64), torch.ones(4)
+    for args in ((None, pos, f), (x, None, f), (x, pos, None)):
+        with pytest.raises(TypeError):
+            call(*args)
