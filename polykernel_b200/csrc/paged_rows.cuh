@@ -20,12 +20,14 @@
 // tensor work (8 cycles per mma.sync and sub-partition) comes near the time of the
 // reads, and P is rounded once to the inputs' type, as in the tile kernel.
 //
+// Values that are not finite are kept out of the loop: see mark_values.
+//
 // Measured (8 key heads of 128, groups of 4, bf16): 64 sequences of up to 16k
-// keys, 2.2 GB, in 388 to 403 us: 5.5 to 5.7 TB/s, where a kernel that only reads
-// reaches 5.2. One token over 4096 keys takes 12.3 us, of which the reads are 2.6:
-// two launches, the cut of the line, one tile's latency and the join. With 48
-// rows of 64-wide heads the chain of a tile (S, softmax, P.V: 3100 cycles in one
-// warp, two to a sub-partition) bounds it: 53 us against 15 for the reads.
+// keys, 2.2 GB, in 333 us: 6.6 TB/s, the rate of a copy. One token over 4096 keys takes
+// 11.2 us on the GPU (14 for a call among others), of which the reads are 2.6: two
+// launches, the cut of the line, one tile's latency and the join. With 48 rows of
+// 64-wide heads the chain of a tile (S, softmax, P.V, in one warp, two to a
+// sub-partition) bounds it: 42 us on the GPU against 15 for the reads.
 #pragma once
 
 #include "paged_common.cuh"

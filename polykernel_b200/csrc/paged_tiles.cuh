@@ -25,18 +25,22 @@
 //   (warp 15 completes a warpgroup.)
 // TMEM: S/P of A [0,128), of B [128,256), O of A [256,384), of B [384,512).
 //
-// P is rounded once to the inputs' type (bf16: 2^-9 relative, fp16: 2^-12),
-// the operand type that the tensor cores take with V; the errors of the keys
-// are independent, so the output's stays at the level of its own rounding.
-// The row sums are of the unrounded P, in fp32.
+// P is rounded once to the inputs' type (by at most 2^-8 of it in bf16, 2^-11 in
+// fp16), the operand type that the tensor cores take with V: an error of at most
+// that share of sum p |v|, and where weights differ, whose errors then add up like
+// independent ones, about as much as the output's own rounding (2.3e-3 in all on
+// normal data, where rounding the exact output gives 1.7e-3). Two terms per weight, as with
+// few rows, would double the tensor work of P.V. The row sums are of the
+// unrounded P, in fp32.
 //
-// Measured (bf16, 128-wide heads): an 8190-token prompt of 32 heads on 8 key heads
-// 530 us, 1037 TFLOP/s (0.64 of the burst matrix rate, 0.76 of the sustained one;
-// the run is power capped at 1.7 GHz); 4 x 32 heads x 2048 tokens over 4096 keys 450
-// us, 917 TFLOP/s; 509 tokens of 28 heads on 4 over 130k keys 959 us, 991 TFLOP/s. A
-// key tile takes a pair of row tiles 3400 cycles: their chains (S, softmax, P.V,
-// and the hand-overs between) alternate, and the tensor pipe waits a third of
-// the time; an item's begin and end cost 5000 to 9000 cycles more.
+// Measured (bf16, 128-wide heads, two cards): an 8190-token prompt of 32 heads on 8
+// key heads 540 to 549 us, 1000 to 1018 TFLOP/s (0.63 of the burst matrix rate, 0.74 of the
+// sustained one; the run is power capped at 1.7 GHz); 4 x 32 heads x 2048 tokens over
+// 4096 keys 464 to 474 us, 870 to 889 TFLOP/s; 509 tokens of 28 heads on 4 over 130k keys
+// 967 to 989 us, 961 to 983 TFLOP/s. A key tile takes a pair of row tiles 3400 cycles: their
+// chains (S, softmax, P.V, and the hand-overs between) alternate, and the tensor pipe
+// waits nearly half of the time (54% active); an item's begin and end cost 5000 to 9000
+// cycles more.
 //
 // With few row tiles over a long cache, `splits` items share a tile's keys and
 // paged_join_kernel adds their pieces up.

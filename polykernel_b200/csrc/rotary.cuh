@@ -16,9 +16,10 @@
 // below: its phases ran one after the other), and registers are kept to four to
 // six blocks per SM, for the loads in flight that the bandwidth needs.
 // Measured: 4 x 32 x 2048 x 128 bf16 rotated in 25.6 us (5.2 TB/s, 0.80 of the
-// copy rate), 5003 x 24 x 96 fp32 in 18.8 us (4.9 TB/s); 15618 tokens of 16 ragged
-// chunks, q and k rotated, appended in 68 us (5.7 TB/s); 16381 tokens of 16 heads of 64,
-// only moved, in 30.5 us (4.4 TB/s: rows of 128 bytes, each to a line of its own).
+// copy rate), 5003 x 24 x 96 fp32 in 18.5 us (5.0 TB/s); 15618 tokens of 16 ragged
+// chunks, q and k rotated, appended in 70 us (5.5 TB/s); 16381 tokens of 16 heads of 64,
+// only moved, in 30 us (4.5 TB/s: a warp's rows are the heads of few tokens, and go to
+// places a page apart).
 #pragma once
 
 #include "paged_index.h"
@@ -78,8 +79,11 @@ __device__ __forceinline__ void item_offsets(const RowShape& s, int item, int& u
 // 64 bits and reduced there: position * frequency has no fraction left in 32
 // bits once it passes 2^24 radians, and only 8 bits of one at 2^16. For 16-bit
 // values the reduced angle goes to the SFU, whose error on [-pi, pi], 2^-21.4,
-// is far below their rounding (2^-9 and 2^-12); the accurate functions took
-// more instructions than everything else together.
+// is far below their rounding (2^-8 and 2^-11); the accurate functions took
+// more instructions than everything else together. Rounding the reduced part to 32
+// bits (by at most 2^-26 of a turn, 2^-23.3 radians) is less than the sine's own error for
+// 16-bit values, and moves fp32 ones by at most 2^-23.3 of their pair (5.5e-8 in all on
+// normal data, where 32-bit products with cosines rounded from 64 bits have 3.9e-8).
 template <typename T, int P>
 __device__ __forceinline__ void angles(const float* __restrict__ inv_freq, long long position, float factor,
                                        bool backward, float (&c)[P], float (&s)[P]) {
