@@ -44,3 +44,28 @@ def test_late_tiles_end_the_call(cuda, case):
     assert codes[:3] == [4] * 3
     assert torch.equal(pk.ops.paged_attention(*args, max_q_len=most)[:n], want)
     assert pk.device_error() == 0
+
+
+@pytest.mark.gpu
+def test_going_over_values_again_is_no_late_tile(cuda):
+    """Where values are not finite, blocks go over a run's values once more, for
+    longer than a wait may last: the fetching warp's limit runs anew meanwhile."""
+    import math
+
+    import polykernel_b200 as pk
+    lib = pk.lib()
+    B, total, page = 40, 8000, 64
+    q, kp, vp, table, cu, lens = args = make([1] * B, [total] * B, page, 4, 4, 128, torch.bfloat16)
+    vp[table[:, 0].long(), :, 5, 3] = math.inf
+    vp[table[:, 90].long(), :, 0, 70] = -math.inf
+    want = pk.ops.paged_attention(*args, max_q_len=1)[:B].clone()
+    assert bool((want[..., 3] == math.inf).all()) and bool((want[..., 70] == -math.inf).all())
+    assert int((~torch.isfinite(want)).sum()) == 2 * want.shape[0] * want.shape[1]
+    try:
+        assert lib.pkb200_selftest_paged_limits(200_000, 0) == 0  # ~0.1 ms
+        for _ in range(3):
+            got = pk.ops.paged_attention(*args, max_q_len=1)[:B]
+            torch.cuda.synchronize()
+            assert pk.device_error() == 0 and torch.equal(got, want)
+    finally:
+        lib.pkb200_selftest_paged_limits(0, 0)
